@@ -526,6 +526,48 @@ ESA_API int esa_weight_grad(long long rows, int n, const void* const* g, const v
                    void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Varlen attention with a learned bias by relative position (no counterpart */
+/* in the reference): the scores of esa_varlen_attn_fwd with ESA_MASK_NONE    */
+/* plus table[bucket(d)][head], d = (j - first key of the segment) - (i -     */
+/* first query of the segment) - q_start[segment] for key token j and query   */
+/* token i (q_start null: 0; offsets beyond +-2^30 count as that).            */
+/*                                                                           */
+/* table [num_buckets, heads] of table_dtype (ESA_F32 or ESA_BF16).           */
+/* bucket_starts: a host array of num_starts ascending distances, the first   */
+/* 0, the last at most 768: the buckets of one side, each from its start up   */
+/* to the next one's, the last without end.  num_starts == num_buckets: keys  */
+/* before the query (distance -d), every key after it in bucket 0.            */
+/* 2 num_starts == num_buckets: both sides, keys after the query (d > 0) in   */
+/* the upper num_starts buckets.  num_starts <= 128.                          */
+/*                                                                           */
+/* A table entry of -inf leaves its pairs out; finite ones beyond +-1e4 count */
+/* as +-1e4.  A query without a key gets output 0 and lse -inf, and so does a */
+/* token in no segment.  Tensors, dtypes, head dims, dropout and lse are      */
+/* those of esa_varlen_attn_fwd, but up to 2^29 - 1 tokens of any row size.   */
+/* dtable [num_buckets, heads] fp32: sums of dS in a fixed order              */
+/* (deterministic; for bf16 calls their row statistic comes from the rounded  */
+/* output, relative error about 2^-10).  Workspace size from the query.       */
+/* ------------------------------------------------------------------------ */
+ESA_API int esa_rel_attn_workspace_size(int batch, int total_q, int total_k, int heads, int head_dim,
+                   int dtype, int num_buckets, const int* bucket_starts, int num_starts,
+                   int backward, size_t* bytes);
+ESA_API int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table,
+                   int table_dtype, int num_buckets, const int* bucket_starts, int num_starts,
+                   const int* q_start, const int* cu_seqlens_q, const int* cu_seqlens_k,
+                   int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
+                   float softmax_scale, float dropout_p, unsigned long long dropout_seed,
+                   void* out, float* softmax_lse, void* workspace, size_t workspace_bytes,
+                   void* stream);
+ESA_API int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                   const void* out, const float* softmax_lse, const void* table,
+                   int table_dtype, int num_buckets, const int* bucket_starts, int num_starts,
+                   const int* q_start, const int* cu_seqlens_q, const int* cu_seqlens_k,
+                   int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
+                   float softmax_scale, float dropout_p, unsigned long long dropout_seed,
+                   void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Profiling hook (no counterpart in the reference; used by the benchmark).  */
 /* While enabled, every kernel launch of the entry points above is           */
 /* bracketed by hipEvents on its stream.  esa_profile_collect waits for the  */

@@ -8,6 +8,7 @@ point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -115,6 +116,18 @@ _PROTOS = {
     "esa_weight_grad": (_c_int, [_c_i64, _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_c_int),
                                  ctypes.POINTER(_c_int), _c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), _vp, _c_sz,
                                  _vp]),
+    # batch tq tk heads hd dtype | buckets starts n_starts | backward bytes
+    "esa_rel_attn_workspace_size": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                             ctypes.POINTER(_c_int), _c_int, _c_int, ctypes.POINTER(_c_sz)]),
+    # q k v | table dtype buckets starts n_starts q_start | cu_q cu_k batch tq tk heads hd dtype | scale dropout_p seed |
+    # out lse ws bytes stream
+    "esa_rel_attn_fwd": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int, _vp, _vp, _vp,
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp, _vp,
+                                  _c_sz, _vp]),
+    # dout q k v out lse | as the forward | dq dk dv dtable ws bytes stream
+    "esa_rel_attn_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int, _vp,
+                                  _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp,
+                                  _vp, _vp, _vp, _c_sz, _vp]),
     "esa_mab_residual_fwd": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _vp, _vp]),
     "esa_mab_residual_bwd": (_c_int, [_vp, _vp, _c_i64, _c_int, _vp, _vp, _vp]),
     "esa_profile_enable": (_c_int, [_c_int]),
@@ -165,6 +178,19 @@ def require_gpu(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise EsaError("the MI355X kernels take device tensors; got a tensor on " + str(t.device))
+
+
+def require_one_device(*tensors: torch.Tensor) -> None:
+    first = tensors[0].device
+    for t in tensors[1:]:
+        if t.device != first:
+            raise EsaError(f"tensors on different devices: {first} and {t.device}")
+
+
+def on_device(t: torch.Tensor):
+    """The context in which a kernel over t is launched: t's device as the current one (a stream takes launches of its
+    own device alone)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

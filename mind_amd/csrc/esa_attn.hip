@@ -61,6 +61,7 @@
 #include "esa_common.h"
 #include "esa_graph_attn.h"
 #include "esa_profile.h"
+#include "esa_rel_bias.h"
 #include "../../include/esa_hip.h"
 
 namespace {
@@ -1353,6 +1354,7 @@ struct AttnF32Args {
   const int4* plan;         // (outer begin, outer segment end, partner begin, partner end) per group
   const int* count;         // number of groups
   float* o; float* lse_out; float* dq; float* dk; float* dv;
+  RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
 };
 
 // Rows of HD fp32 values (HD = 16, 24, 32 or 64) as float4 chunks.
@@ -1591,7 +1593,7 @@ DEVI void f32_stages(int lo, int hi, bool live, Load load, Store store, Use use)
   }
 }
 
-template <bool MASKED, int HD, bool DROP>
+template <bool MASKED, int HD, bool DROP, bool BIAS = false>
 __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 1 : 4))) void attn_fwd_f32_kernel(const AttnF32Args a) {
   using T = F32Tile<HD>;
@@ -1619,6 +1621,8 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
     m[b] = -INFINITY;
     l[b] = 0.f;
   }
+  const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line(sRel, a.rel, head, tid, T::kThreads);
   f32x4 rK[T::kPer], rV[T::kPer];
   int2 rN = make_int2(-1, -1);
   uint32_t rKey = 0;
@@ -1646,6 +1650,19 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
           for (int b = 0; b < QB; ++b) s[kb][b] = f32_product<HD>(x, q[b]);
         }
         const bool tail = k0 + kF32Stage > phi;
+        if (BIAS) {
+          const int base = rel_base(a.rel, k0, first, shift);
+          bool far_hi;
+          const bool near = rel_near(a.rel, base, kF32Stage, 16 * QB, far_hi);
+          const float* line = sRel + base + 4 * grp - c16;
+          const float far = sRel[far_hi ? a.rel.stride - 1 : 0];
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[kb][b][r] = fmaf(s[kb][b][r], a.c, near ? line[16 * (kb - b) + r] : far);
+        }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -1654,7 +1671,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
             const int2 pn = MASKED ? sN[buf][key] : make_int2(0, 0);
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
-              s[kb][b][r] *= a.c;
+              if (!BIAS) s[kb][b][r] *= a.c;
               if (MASKED || tail)
                 s[kb][b][r] = admissible_f32<MASKED>(k0 + key, phi, own.tok[b], pn, node[b]) ? s[kb][b][r] : -INFINITY;
             }
@@ -1901,7 +1918,7 @@ __global__ __launch_bounds__(256) void attn_dkdv_few_kernel(const AttnFewArgs a)
 }
 
 // dQ = scale * sum_j P_ij (dP_ij - D_i) k_j, P recomputed from the saved LSE.
-template <bool MASKED, int HD, bool DROP>
+template <bool MASKED, int HD, bool DROP, bool BIAS = false>
 __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 4 : 1))) void attn_dq_f32_kernel(const AttnF32Args a) {
   using T = F32Tile<HD>;
@@ -1926,6 +1943,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
 #pragma unroll
     for (int c = 0; c < NR; ++c) acc[b][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     rs[b] = a.rows[(size_t)head * a.tq_pad + own.tok[b]];   // (LSE2, D)
+    if (BIAS && !own.valid[b]) rs[b].x = INFINITY;           // its dS is summed by distance: P = 0
     node[b] = MASKED ? a.nodes[own.tok[b]] : make_int2(0, 0);
     rk[b] = DROP ? drop_row(a.drop, own.tok[b], head) : 0u;
   }
@@ -1933,6 +1951,12 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   int2 rN = make_int2(-1, -1);
   uint32_t rKey = 0;
   bool odd = false;   // edge mask: this thread staged an infinity or a NaN of a key
+  const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
+  RelSums<4> sums(sRel, a.rel.stride, T::kThreads / 64, wave, grp);
+  if (BIAS) {
+    rel_load_line(sRel, a.rel, head, tid, T::kThreads);
+    sums.clear(a.rel.stride, lane);
+  }
   auto walk = [&](auto checked) {
     f32_stages(
         own.plo, phi, own.live,
@@ -1951,6 +1975,11 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
         },
         [&](int buf, int k0) {
           const bool tail = k0 + kF32Stage > phi;
+          const int base = BIAS ? rel_base(a.rel, k0, first, shift) : 0;
+          bool far_hi = false;
+          const bool near = BIAS && rel_near(a.rel, base, kF32Stage, 16 * QB, far_hi);
+          const float far = BIAS ? sRel[far_hi ? a.rel.stride - 1 : 0] : 0.f;
+          float far_sum = 0.f;
           auto block = [&](int kb) {
             f32x4 x[NR], s[QB], ds[QB];
             f32_rows<HD>(x, sK[buf], 16 * kb, c16, grp);
@@ -1965,12 +1994,16 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
               const int2 pn = MASKED ? sN[buf][key] : make_int2(0, 0);
 #pragma unroll
               for (int b = 0; b < QB; ++b) {
-                const float p = fast_exp2(a.c * s[b][r] - rs[b].x);
+                const int entry = base + key - 16 * b - c16;
+                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], near ? sRel[entry] : far) - rs[b].x
+                                               : a.c * s[b][r] - rs[b].x);
                 float dp = ds[b][r];
                 if (DROP) dp = drop_keep(a.drop, rk[b], sKey[buf][key], k0 + key) ? dp * a.drop.inv_keep : 0.f;
                 ds[b][r] = p * (dp - rs[b].y);
                 if (MASKED || tail)
                   ds[b][r] = admissible_f32<MASKED>(k0 + key, phi, own.tok[b], pn, node[b]) ? ds[b][r] : 0.f;
+                if (BIAS && near) sums.add(entry, ds[b][r]);
+                if (BIAS && !near) far_sum += ds[b][r];
               }
             }
             if constexpr (decltype(checked)::value)
@@ -1985,9 +2018,16 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) block(kb);
           }
+          if (BIAS) {
+            if (near) sums.stage_done(base, a.rel.stride, lane);
+            else (far_hi ? sums.hi : sums.lo) += far_sum;
+          }
         });
   };
   walk(std::false_type());
+  if (BIAS)
+    rel_fold(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, T::kThreads / 64, wave, lane, tid,
+             T::kThreads);
   if (MASKED && __syncthreads_or(odd)) {   // again, over the admissible pairs alone
 #pragma unroll
     for (int b = 0; b < QB; ++b)
@@ -2001,7 +2041,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
 }
 
 // dV = sum_i P_ij dO_i, dK = scale * sum_i P_ij (dP_ij - D_i) q_i; the partners are queries with their (LSE2, D).
-template <bool MASKED, int HD, bool DROP>
+template <bool MASKED, int HD, bool DROP, bool BIAS = false>
 __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 4 : 1))) void attn_dkdv_f32_kernel(const AttnF32Args a) {
   using T = F32Tile<HD>;
@@ -2033,6 +2073,8 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   int2 rN = make_int2(-1, -1);
   uint32_t rKey = 0;
   bool odd = false;   // edge mask: this thread staged an infinity or a NaN of a q or dO row
+  const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line(sRel, a.rel, head, tid, T::kThreads);
   auto walk = [&](auto checked) {
     f32_stages(
         own.plo, phi, own.live,
@@ -2060,6 +2102,10 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
           }
         },
         [&](int buf, int q0) {
+          const int base = BIAS ? rel_base(a.rel, first, q0, shift) : 0;
+          bool far_hi = false;
+          const bool near = BIAS && rel_near(a.rel, base, 16 * QB, kF32Stage, far_hi);
+          const float far = BIAS ? sRel[far_hi ? a.rel.stride - 1 : 0] : 0.f;
           auto block = [&](int kb) {
             f32x4 x[NR], s[QB], ds[QB];
             f32_rows<HD>(x, sQ[buf], 16 * kb, c16, grp);
@@ -2075,7 +2121,9 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
               const int2 pn = MASKED ? sN[buf][qi] : make_int2(0, 0);
 #pragma unroll
               for (int b = 0; b < QB; ++b) {
-                const float p = fast_exp2(a.c * s[b][r] - lse2[r]);   // a query past the range has LSE2 = inf
+                // a query past the range has LSE2 = inf
+                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], near ? sRel[base + 16 * b + c16 - qi] : far) - lse2[r]
+                                               : a.c * s[b][r] - lse2[r]);
                 const bool in = !MASKED || admissible_f32<true>(q0 + qi, phi, own.tok[b], pn, node[b]);
                 const bool keep = !DROP || drop_keep(a.drop, sKey[buf][qi], ck[b], own.tok[b]);
                 float dp = ds[b][r];
@@ -2249,6 +2297,13 @@ __global__ __launch_bounds__(256) void prep_kernel(const PrepArgs p) {
   if (b < p.nb[kBoundsK]) { bounds_item(p.cu_k, p.cu_q, p.nseg, p.total_k, p.tk_pad, p.bounds_k, b * 256 + tid); return; }
   b -= p.nb[kBoundsK];
   if (b < p.nb[kRows]) rowstats_item(p, (long)b * 256 + tid);
+}
+
+// The fp32 preparation with a relative position bias; backward: the row statistics behind it.
+__global__ __launch_bounds__(256) void rel_prep_f32_kernel(const RelPrep p, const RelPass r, const PrepArgs rows, int nb) {
+  const int b = blockIdx.x;
+  if (b < nb) rel_prep_block(p, r, b, threadIdx.x);
+  else rowstats_item(rows, (long)(b - nb) * 256 + threadIdx.x);
 }
 
 __global__ void edge_mask_dense_kernel(const int* __restrict__ src, const int* __restrict__ dst,
@@ -2668,6 +2723,37 @@ AttnFewArgs few_args(const void* q, const void* k, const void* v, const int* cu_
     else ESA_F32_LAUNCH_HD(KERNEL, false, hd, grid, st, a);                                         \
   } while (0)
 
+// ---- with a relative position bias (the calls of esa_rel_attn.hip)
+#define ESA_F32_REL_K(KERNEL, HD, D, grid, lds, st, a)                                                             \
+  hipLaunchKernelGGL((KERNEL<false, HD, D, true>), grid, dim3(F32Tile<HD>::kThreads), lds(F32Tile<HD>::kThreads / 64), \
+                     st, a)
+#define ESA_F32_REL_HD(KERNEL, D, hd, grid, lds, st, a)                 \
+  do {                                                                  \
+    if (hd == 16) ESA_F32_REL_K(KERNEL, 16, D, grid, lds, st, a);       \
+    else if (hd == 24) ESA_F32_REL_K(KERNEL, 24, D, grid, lds, st, a);  \
+    else if (hd == 32) ESA_F32_REL_K(KERNEL, 32, D, grid, lds, st, a);  \
+    else ESA_F32_REL_K(KERNEL, 64, D, grid, lds, st, a);                \
+  } while (0)
+#define ESA_F32_REL_LAUNCH(KERNEL, hd, drop, grid, lds, st, a)      \
+  do {                                                              \
+    if (drop) ESA_F32_REL_HD(KERNEL, true, hd, grid, lds, st, a);   \
+    else ESA_F32_REL_HD(KERNEL, false, hd, grid, lds, st, a);       \
+  } while (0)
+
+AttnF32Args f32_rel_args(const DenseAttnCall& c, const RelPass& r) {
+  AttnF32Args a{};
+  a.q = static_cast<const float*>(c.q); a.k = static_cast<const float*>(c.k); a.v = static_cast<const float*>(c.v);
+  a.total_q = c.total_q; a.total_k = c.total_k; a.heads = c.heads; a.tq_pad = r.tq_pad;
+  a.c = c.scale * kLog2e; a.scale = c.scale;
+  a.drop = c.drop;
+  a.rel = r.bias;
+  a.plan = r.plan_q; a.count = r.count_q; a.shift = r.shift_q;
+  return a;
+}
+dim3 f32_rel_grid(int total, const DenseAttnCall& c) {
+  return dim3((unsigned)(groups_of(total) + std::min(c.nseg, total)) * (unsigned)c.heads);
+}
+
 // Scratch of esa_varlen_attn_fwd_noalloc: a file-scope device array, one
 // copy per GPU, held until the process ends.  Host code never passes the
 // array's name (a host-side stand-in) to a kernel: it passes the device
@@ -2698,6 +2784,49 @@ int scratch_address(void** out) {
 }
 
 }  // namespace
+
+int f32_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            hipLaunchKernelGGL(rel_prep_f32_kernel, dim3(nb), dim3(256), 0, st, p, r, PrepArgs{}, nb));
+  ESA_LAUNCH_CHECK();
+  if (c.total_q == 0) return ESA_OK;
+  AttnF32Args a = f32_rel_args(c, r);
+  a.o = static_cast<float*>(c.out); a.lse_out = c.lse;
+  auto lds = [&](int) { return r.bias.stride * sizeof(float); };
+  ESA_TIMED(esa_profile::kAttnFwd, st,
+            ESA_F32_REL_LAUNCH(attn_fwd_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c), lds, st, a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+int f32_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
+  PrepArgs rows{};
+  rows.total_q = c.total_q; rows.heads = c.heads; rows.tq_pad = r.tq_pad; rows.head_dim = c.head_dim;
+  rows.lse = c.lse_in; rows.rows_f = r.rows;
+  rows.dout_f = static_cast<const float*>(c.dout); rows.out_f = static_cast<const float*>(c.out_in);
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            hipLaunchKernelGGL(rel_prep_f32_kernel, dim3(nb + blocks_for((long)c.heads * r.tq_pad)), dim3(256), 0, st, p, r,
+                               rows, nb));
+  ESA_LAUNCH_CHECK();
+  AttnF32Args a = f32_rel_args(c, r);
+  a.out = static_cast<const float*>(c.out_in); a.dout = static_cast<const float*>(c.dout);
+  a.rows = r.rows;
+  a.dq = static_cast<float*>(c.dq); a.dk = static_cast<float*>(c.dk); a.dv = static_cast<float*>(c.dv);
+  auto line = [&](int) { return r.bias.stride * sizeof(float); };
+  auto sums = [&](int waves) { return rel_dq_floats(r.bias.stride, waves, 4) * sizeof(float); };
+  if (c.total_q > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDq, st,
+              ESA_F32_REL_LAUNCH(attn_dq_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c), sums, st, a));
+  ESA_LAUNCH_CHECK();
+  a.plan = r.plan_k; a.count = r.count_k; a.shift = r.shift_k;
+  if (c.total_k > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
+              ESA_F32_REL_LAUNCH(attn_dkdv_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_k, c), line, st, a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
 
 extern "C" {
 

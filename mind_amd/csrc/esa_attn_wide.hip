@@ -48,6 +48,7 @@
 #include "esa_attn_tiles.h"
 #include "esa_attn_dense.h"
 #include "esa_profile.h"
+#include "esa_rel_bias.h"
 #include "../../include/esa_hip.h"
 
 namespace {
@@ -79,6 +80,7 @@ struct WideArgs {
   int total_q, total_k, heads, tq_pad;
   float c, scale;
   bf16* o; float* lse_out; bf16* dq; bf16* dk; bf16* dv;
+  RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
 };
 
 // LDS position of staged token t in octet o of an NO-octet layout.  The
@@ -181,9 +183,10 @@ struct WStage {
   i32x4 r[CPT];
 };
 
-template <int HD>
+// CUT: tokens at or past `end` become zero rows; whatever the next segment holds, a zero weight times it stays zero.
+template <int HD, bool CUT = false>
 DEVI WStage<HD> wide_gload(const bf16* a, const bf16* b, int g0, int total, int H, int head, int tid,
-                           int lo = INT_MIN) {
+                           int lo = INT_MIN, int end = 0) {
   constexpr int NR = HD / 8;
   WStage<HD> s;
 #pragma unroll
@@ -194,6 +197,7 @@ DEVI WStage<HD> wide_gload(const bf16* a, const bf16* b, int g0, int total, int 
     const int tok = rem / NR, o = rem - tok * NR;
     const int t = min(max(g0 + tok, lo), total - 1);
     s.r[i] = *reinterpret_cast<const i32x4*>((tensor ? b : a) + ((size_t)t * H + head) * HD + 8 * o);
+    if (CUT && g0 + tok >= end) s.r[i] = i32x4{};
   }
   return s;
 }
@@ -307,8 +311,25 @@ DEVI void wide_walk(int n_stages, Load gload, Store lstore, Compute compute) {
 
 constexpr int kWGroup = kWaves * kTile;   // 128 owned tokens per block
 
+// x[r] = c s[r] + bias - sub of a 32 x 32 tile whose keys (queries) lie in the registers: entry base + at + 16 (r / 8)
+// + r % 8 of the line, or one value for the tile.
+DEVI bool rel_scores(const RelBias& rel, const float* line, int base, int at, const f32x16& s, float c, float sub,
+                     float (&x)[16]) {
+  bool far_hi;
+  if (rel_near(rel, base, kTile, kTile, far_hi)) {
+    const float* b = line + base + at;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(s[r], c, b[16 * (r >> 3) + (r & 7)] - sub);
+    return true;
+  }
+  const float b = line[far_hi ? rel.stride - 1 : 0] - sub;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = fmaf(s[r], c, b);
+  return false;
+}
+
 // ------------------------------------------------------------------ forward
-template <int HD, bool DROP>
+template <int HD, bool DROP, bool BIAS>
 __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
   __shared__ __align__(16) bf16 sK[2][NO * kWTokPad * 8];
@@ -340,7 +361,8 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) qq = fmaf((float)qop[c][e], (float)qop[c][e], qq);
   qq += __shfl_xor(qq, 32);
-  const float bnd = valid ? a.c * sqrtf(qq) * km : 0.f;
+  float bnd = valid ? a.c * sqrtf(qq) * km : 0.f;
+  if (BIAS) bnd += a.rel.top[head];
   const bool fixed_ref = __builtin_amdgcn_readfirstlane((int)(wave_max(bnd) <= kStaticBound)) != 0;
   f32x16 acc[NM];
 #pragma unroll
@@ -351,13 +373,15 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
   const int n_tiles = (g.w - z0 + kTile - 1) >> 5;
   const int n_stages = (n_tiles + 1) >> 1;
   const f32x16 zero = {};
+  const int shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line(sRel, a.rel, head, tid, 256);
   auto run = [&](auto online_tag) {
   constexpr bool ONLINE = decltype(online_tag)::value;
   wide_walk(
       n_stages,
       [&](int st) {
         WStageK<HD> s;
-        s.rows = wide_gload<HD>(a.k, a.v, z0 + st * kWStage, a.total_k, H, head, tid, DROP ? g.z : INT_MIN);
+        s.rows = wide_gload<HD, BIAS>(a.k, a.v, z0 + st * kWStage, a.total_k, H, head, tid, DROP ? g.z : INT_MIN, g.w);
         s.key = DROP && tid < kWStage ? drop_col(a.drop, z0 + st * kWStage + tid) : 0u;
         return s;
       },
@@ -380,7 +404,31 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
               s[r] = (unsigned)(k0 + row_local(r, h) - g.z) < (unsigned)(g.w - g.z) ? s[r] : -INFINITY;
           }
           float p[16];
-          if (ONLINE) {
+          if (BIAS) {   // scores and m_run in powers of two, c s + bias log2(e)
+            rel_scores(a.rel, sRel, rel_base(a.rel, k0, g.x + wave * kTile, shift), 8 * h - col, s, a.c, 0.f, p);
+            if (ONLINE) {
+              float mt = p[0];
+#pragma unroll
+              for (int r = 1; r < 16; ++r) mt = fmaxf(mt, p[r]);
+              mt = fmaxf(mt, __shfl_xor(mt, 32));
+              const float m_new = fmaxf(m_run, mt);
+              if (__ballot(m_new > m_run)) {
+                const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
+                l_run *= alpha;
+#pragma unroll
+                for (int m = 0; m < NM; ++m)
+#pragma unroll
+                  for (int r = 0; r < 16; ++r) acc[m][r] *= alpha;
+                m_run = m_new;
+              }
+              const float cm = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p[r] = fast_exp2(p[r] - cm);
+            } else {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p[r] = fast_exp2(p[r]);
+            }
+          } else if (ONLINE) {
             float mt = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
@@ -424,14 +472,16 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
   if (!valid) return;
   const float l = l_run + __shfl_xor(l_run, 32);
   store_acc<HD>(a.o + ((size_t)t * H + head) * HD, acc, l > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / l : 0.f, h);
-  if (h == 0) a.lse_out[(size_t)head * a.total_q + t] = l > 0.f ? (a.c * m_run + fast_log2(l)) * kLn2 : -INFINITY;
+  if (h == 0)
+    a.lse_out[(size_t)head * a.total_q + t] =
+        l > 0.f ? ((BIAS ? m_run : a.c * m_run) + fast_log2(l)) * kLn2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------ dQ pass
 // Queries on lanes: S^T = K q^T, dP^T = V dO^T, P = exp2(c S - LSE2),
 // dS = P (dP - D), dQ^T += K^T dS^T.  Also writes the dK/dV pass's row
 // statistics {-LSE2 / c, -D} of its queries.
-template <int HD, bool DROP>
+template <int HD, bool DROP, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && !DROP ? ESA_WIDE_WAVES_DQ64 : 1)))
 void wide_dq_kernel(const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
@@ -461,7 +511,8 @@ void wide_dq_kernel(const WideArgs a) {
   wide_zero_pad<HD>(sK[0], sK[1], sV[0], sV[1], tid);
   dsum += __shfl_xor(dsum, 32);
   const float lq = a.lse[(size_t)head * a.total_q + (valid ? t : g.x)];
-  const float lse2 = lq == -INFINITY ? INFINITY : lq * kLog2e;   // rows without keys: P = 0
+  // rows without keys, and with a bias the lanes past the segment's end (their dS is summed by distance): P = 0
+  const float lse2 = lq == -INFINITY || (BIAS && !valid) ? INFINITY : lq * kLog2e;
   if (valid && h == 0)
     a.aux[(size_t)head * a.tq_pad + t] = make_float2(lq == -INFINITY ? kDeadRow : -lse2 / a.c, -dsum);
   const uint32_t rk = DROP ? drop_row(a.drop, valid ? t : g.x, head) : 0u;
@@ -473,11 +524,17 @@ void wide_dq_kernel(const WideArgs a) {
   const int n_tiles = (g.w - z0 + kTile - 1) >> 5;
   const int n_stages = (n_tiles + 1) >> 1;
   const f32x16 zero = {};
+  const int shift = BIAS ? a.shift[item] : 0;
+  RelSums<2> sums(sRel, a.rel.stride, kWaves, wave, h);
+  if (BIAS) {
+    rel_load_line(sRel, a.rel, head, tid, 256);
+    sums.clear(a.rel.stride, lane);
+  }
   wide_walk(
       n_stages,
       [&](int st) {
         WStageK<HD> s;
-        s.rows = wide_gload<HD>(a.k, a.v, z0 + st * kWStage, a.total_k, H, head, tid, DROP ? g.z : INT_MIN);
+        s.rows = wide_gload<HD, BIAS>(a.k, a.v, z0 + st * kWStage, a.total_k, H, head, tid, DROP ? g.z : INT_MIN, g.w);
         s.key = DROP && tid < kWStage ? drop_col(a.drop, z0 + st * kWStage + tid) : 0u;
         return s;
       },
@@ -487,6 +544,8 @@ void wide_dq_kernel(const WideArgs a) {
       },
       [&](int buf, int st) {
         if (!active) return;
+        const int base = BIAS ? rel_base(a.rel, z0 + st * kWStage, g.x + wave * kTile, shift) : 0;
+        bool any_near = false;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           if (2 * st + u >= n_tiles) break;
@@ -503,23 +562,40 @@ void wide_dq_kernel(const WideArgs a) {
               s[r] = (unsigned)(k0 + row_local(r, h) - g.z) < (unsigned)(g.w - g.z) ? s[r] : -INFINITY;
           }
           float ds[16];
+          bool near = false;
+          if (BIAS) near = rel_scores(a.rel, sRel, base + u * kTile, 8 * h - col, s, a.c, lse2, ds);
           if (DROP) {
             float dpk[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) dpk[r] = dp[r] * a.drop.inv_keep;
             drop_tile(a.drop, rk, &sKey[buf][u * kTile], h, dpk);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = fast_exp2(fmaf(s[r], a.c, -lse2)) * (dpk[r] - dsum);
+            for (int r = 0; r < 16; ++r)
+              ds[r] = fast_exp2(BIAS ? ds[r] : fmaf(s[r], a.c, -lse2)) * (dpk[r] - dsum);
           } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = fast_exp2(fmaf(s[r], a.c, -lse2)) * (dp[r] - dsum);
+            for (int r = 0; r < 16; ++r) ds[r] = fast_exp2(BIAS ? ds[r] : fmaf(s[r], a.c, -lse2)) * (dp[r] - dsum);
+          }
+          if (BIAS) {
+            if (near) {
+              any_near = true;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sums.add(base + u * kTile + 8 * h - col + 16 * (r >> 3) + (r & 7), ds[r]);
+            } else {
+              float x = 0.f;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) x += ds[r];
+              (base + u * kTile > a.rel.reach + kRelPad ? sums.hi : sums.lo) += x;
+            }
           }
 #pragma unroll
           for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[m] = mfma32(tr_dims<NO>(sK[buf], m, 2 * u + j, lane), cvt8(ds + 8 * j), acc[m]);
         }
+        if (BIAS && any_near) sums.stage_done(base, a.rel.stride, lane);
       });
+  if (BIAS) rel_fold(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, kWaves, wave, lane, tid, 256);
   if (!valid) return;
   store_acc<HD>(a.dq + ((size_t)t * H + head) * HD, acc, a.scale, h);
 }
@@ -529,7 +605,7 @@ void wide_dq_kernel(const WideArgs a) {
 // (the row statistics as accumulator seeds), P = exp2(c S), dS = P dP,
 // dV^T += dO^T P, dK^T += Q^T dS.  A stage holds 64 queries' Q and dO rows
 // and their statistics.
-template <int HD, bool DROP>
+template <int HD, bool DROP, bool BIAS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ESA_WIDE_WAVES_DKDV > 0 ? ESA_WIDE_WAVES_DKDV : 1)))
 void wide_dkdv_kernel(const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
@@ -564,13 +640,16 @@ void wide_dkdv_kernel(const WideArgs a) {
   const int n_tiles = (g.w - g.z + kTile - 1) >> 5;
   const int n_stages = (n_tiles + 1) >> 1;
   struct Stage { WStage<HD> rows; float2 st; uint32_t key; };
+  const int shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line(sRel, a.rel, head, tid, 256);
   wide_walk(
       n_stages,
       [&](int st) {
         Stage s;
-        s.rows = wide_gload<HD>(a.q, a.dout, g.z + st * kWStage, a.total_q, H, head, tid);
+        s.rows = wide_gload<HD, BIAS>(a.q, a.dout, g.z + st * kWStage, a.total_q, H, head, tid, INT_MIN, g.w);
         const int qi = g.z + st * kWStage + tid;
         s.st = tid < kWStage ? a.aux[(size_t)head * a.tq_pad + min(qi, a.tq_pad - 1)] : make_float2(0.f, 0.f);
+        if (BIAS && qi >= g.w) s.st = make_float2(kDeadRow, 0.f);
         s.key = DROP && tid < kWStage ? drop_row(a.drop, qi, head) : 0u;
         return s;
       },
@@ -609,7 +688,20 @@ void wide_dkdv_kernel(const WideArgs a) {
           }
           float p[16], ds[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) p[r] = fast_exp2(s[r] * a.c);
+          for (int r = 0; r < 16; ++r) p[r] = BIAS ? 0.f : fast_exp2(s[r] * a.c);
+          if (BIAS) {   // the queries lie in the registers: distances fall as r rises
+            const int base = rel_base(a.rel, x0 + wave * kTile, q0, shift);
+            bool far_hi;
+            if (rel_near(a.rel, base, kTile, kTile, far_hi)) {
+              const float* b = sRel + base + col - 8 * h;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[r], a.c, b[-(16 * (r >> 3) + (r & 7))]));
+            } else {
+              const float b = sRel[far_hi ? a.rel.stride - 1 : 0];
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[r], a.c, b));
+            }
+          }
           if (q0 + kTile > g.w) {   // the segment's last, partial query tile
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = q0 + row_local(r, h) < g.w ? p[r] : 0.f;
@@ -731,6 +823,14 @@ __global__ __launch_bounds__(256) void wide_prep_kernel(const WidePrep p) {
   }
 }
 
+// The same with a relative position bias: its preparation, then (forward) the key norms.
+template <int HD>
+__global__ __launch_bounds__(256) void wide_rel_prep_kernel(const RelPrep p, const RelPass r, const WidePrep w, int nb) {
+  const int b = blockIdx.x;
+  if (b < nb) rel_prep_block(p, r, b, threadIdx.x);
+  else wide_knorm_block<HD>(w, b - nb, threadIdx.x);
+}
+
 size_t wal256(size_t x) { return (x + 255) & ~size_t(255); }
 int wr32(int x) { return (x + kTile - 1) / kTile * kTile; }
 // Groups of one direction: at most ceil(T / 128) + (non-empty segments) <= ceil(T / 128) + T.
@@ -756,25 +856,31 @@ unsigned wide_grid(int total_outer, int nseg, int heads) {
   return (unsigned)(((total_outer + kWGroup - 1) / kWGroup + min(nseg, total_outer)) * heads);
 }
 
-#define ESA_WIDE_LAUNCH_HD(KERNEL, D, hd, grid, st, a)                                   \
-  do {                                                                                    \
-    if (hd == 16) hipLaunchKernelGGL((KERNEL<16, D>), grid, dim3(256), 0, st, a);         \
-    else if (hd == 24) hipLaunchKernelGGL((KERNEL<24, D>), grid, dim3(256), 0, st, a);    \
-    else if (hd == 32) hipLaunchKernelGGL((KERNEL<32, D>), grid, dim3(256), 0, st, a);    \
-    else hipLaunchKernelGGL((KERNEL<64, D>), grid, dim3(256), 0, st, a);                  \
+#define ESA_WIDE_LAUNCH_HD(KERNEL, D, B, hd, grid, lds, st, a)                              \
+  do {                                                                                       \
+    if (hd == 16) hipLaunchKernelGGL((KERNEL<16, D, B>), grid, dim3(256), lds, st, a);       \
+    else if (hd == 24) hipLaunchKernelGGL((KERNEL<24, D, B>), grid, dim3(256), lds, st, a);  \
+    else if (hd == 32) hipLaunchKernelGGL((KERNEL<32, D, B>), grid, dim3(256), lds, st, a);  \
+    else hipLaunchKernelGGL((KERNEL<64, D, B>), grid, dim3(256), lds, st, a);                \
   } while (0)
-#define ESA_WIDE_PREP(hd, grid, st, p)                                                         \
-  do {                                                                                    \
-    if (hd == 16) hipLaunchKernelGGL((wide_prep_kernel<16>), grid, dim3(256), 0, st, p);  \
-    else if (hd == 24) hipLaunchKernelGGL((wide_prep_kernel<24>), grid, dim3(256), 0, st, p); \
-    else if (hd == 32) hipLaunchKernelGGL((wide_prep_kernel<32>), grid, dim3(256), 0, st, p); \
-    else hipLaunchKernelGGL((wide_prep_kernel<64>), grid, dim3(256), 0, st, p);           \
+#define ESA_WIDE_PREP_K(KERNEL, hd, grid, st, ...)                                            \
+  do {                                                                                         \
+    if (hd == 16) hipLaunchKernelGGL((KERNEL<16>), grid, dim3(256), 0, st, __VA_ARGS__);       \
+    else if (hd == 24) hipLaunchKernelGGL((KERNEL<24>), grid, dim3(256), 0, st, __VA_ARGS__);  \
+    else if (hd == 32) hipLaunchKernelGGL((KERNEL<32>), grid, dim3(256), 0, st, __VA_ARGS__);  \
+    else hipLaunchKernelGGL((KERNEL<64>), grid, dim3(256), 0, st, __VA_ARGS__);                \
   } while (0)
+#define ESA_WIDE_PREP(hd, grid, st, p) ESA_WIDE_PREP_K(wide_prep_kernel, hd, grid, st, p)
 // Head dim 16 only with dropout (without, esa_attn_dense.hip's kernels run).
 #define ESA_WIDE_LAUNCH(KERNEL, hd, drop, grid, st, a)                                   \
   do {                                                                                    \
-    if (drop) ESA_WIDE_LAUNCH_HD(KERNEL, true, hd, grid, st, a);                         \
-    else ESA_WIDE_LAUNCH_HD(KERNEL, false, hd, grid, st, a);                             \
+    if (drop) ESA_WIDE_LAUNCH_HD(KERNEL, true, false, hd, grid, 0, st, a);               \
+    else ESA_WIDE_LAUNCH_HD(KERNEL, false, false, hd, grid, 0, st, a);                   \
+  } while (0)
+#define ESA_WIDE_REL_LAUNCH(KERNEL, hd, drop, grid, lds, st, a)                          \
+  do {                                                                                    \
+    if (drop) ESA_WIDE_LAUNCH_HD(KERNEL, true, true, hd, grid, lds, st, a);              \
+    else ESA_WIDE_LAUNCH_HD(KERNEL, false, true, hd, grid, lds, st, a);                  \
   } while (0)
 
 }  // namespace
@@ -852,6 +958,61 @@ int wide_attn_bwd(const DenseAttnCall& c, void* workspace, size_t workspace_byte
   ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
             ESA_WIDE_LAUNCH(wide_dkdv_kernel, c.head_dim, c.dropout, dim3(wide_grid(c.total_k, c.nseg, c.heads)), st,
                             a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+// ---- with a relative position bias (the calls of esa_rel_attn.hip)
+static WideArgs wide_rel_args(const DenseAttnCall& c, const RelPass& r) {
+  WideArgs a{};
+  a.q = static_cast<const bf16*>(c.q); a.k = static_cast<const bf16*>(c.k); a.v = static_cast<const bf16*>(c.v);
+  a.total_q = c.total_q; a.total_k = c.total_k; a.heads = c.heads; a.tq_pad = r.tq_pad;
+  a.c = c.scale * kLog2e; a.scale = c.scale;
+  a.drop = c.drop;
+  a.rel = r.bias;
+  a.groups = r.plan_q; a.count = r.count_q; a.shift = r.shift_q;
+  return a;
+}
+
+int wide_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
+  WidePrep w{};
+  w.total_k = c.total_k; w.heads = c.heads; w.tk_tiles = r.tk_tiles;
+  w.k = static_cast<const bf16*>(c.k); w.knorm = r.knorm;
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            ESA_WIDE_PREP_K(wide_rel_prep_kernel, c.head_dim, dim3(nb + r.tk_tiles), st, p, r, w, nb));
+  ESA_LAUNCH_CHECK();
+  if (c.total_q == 0) return ESA_OK;
+  WideArgs a = wide_rel_args(c, r);
+  a.knorm = r.knorm; a.tk_tiles = r.tk_tiles;
+  a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
+  const dim3 grid(wide_grid(c.total_q, c.nseg, c.heads));
+  ESA_TIMED(esa_profile::kAttnFwd, st,
+            ESA_WIDE_REL_LAUNCH(wide_fwd_kernel, c.head_dim, c.dropout, grid, r.bias.stride * sizeof(float), st, a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+int wide_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            hipLaunchKernelGGL((wide_rel_prep_kernel<16>), dim3(nb), dim3(256), 0, st, p, r, WidePrep{}, nb));
+  ESA_LAUNCH_CHECK();
+  WideArgs a = wide_rel_args(c, r);
+  a.out = static_cast<const bf16*>(c.out_in); a.dout = static_cast<const bf16*>(c.dout);
+  a.lse = c.lse_in; a.aux = r.rows;
+  a.dq = static_cast<bf16*>(c.dq); a.dk = static_cast<bf16*>(c.dk); a.dv = static_cast<bf16*>(c.dv);
+  const size_t line = r.bias.stride * sizeof(float);
+  if (c.total_q > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDq, st,
+            ESA_WIDE_REL_LAUNCH(wide_dq_kernel, c.head_dim, c.dropout, dim3(wide_grid(c.total_q, c.nseg, c.heads)),
+                                rel_dq_floats(r.bias.stride, kWaves, 2) * sizeof(float), st, a));
+  ESA_LAUNCH_CHECK();
+  a.groups = r.plan_k; a.count = r.count_k; a.shift = r.shift_k;
+  if (c.total_k > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
+            ESA_WIDE_REL_LAUNCH(wide_dkdv_kernel, c.head_dim, c.dropout, dim3(wide_grid(c.total_k, c.nseg, c.heads)),
+                                line, st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }

@@ -1,0 +1,211 @@
+// Entry points of the varlen attention with a learned bias by relative
+// position: argument checks, the workspace, the last sum of the table's
+// gradient.  The passes are the unmasked kernels' own (esa_attn_wide.hip for
+// bf16, esa_attn.hip for fp32); esa_rel_bias.h has the bias.
+#include <algorithm>
+
+#include "esa_rel_bias.h"
+#include "esa_profile.h"
+#include "../../include/esa_hip.h"
+
+namespace {
+
+// dtable[b][h] = the sum of part[group][h][b] over the call's groups.  A block
+// takes 32 columns of part; its 32 rows of threads sum every 32nd group each
+// and are then added in order.
+constexpr int kReduceCols = 32, kReduceRows = 32;
+__global__ __launch_bounds__(kReduceCols* kReduceRows) void rel_reduce_kernel(const float* __restrict__ part,
+                                                                              const int* __restrict__ count, int heads,
+                                                                              int buckets, float* __restrict__ dtable) {
+  __shared__ float s[kReduceRows][kReduceCols + 1];
+  const int x = threadIdx.x % kReduceCols, y = threadIdx.x / kReduceCols;
+  const int cols = heads * buckets, c = blockIdx.x * kReduceCols + x, n = *count;
+  float sum = 0.f;
+  if (c < cols)
+    for (int i = y; i < n; i += kReduceRows) sum += part[(size_t)i * cols + c];
+  s[y][x] = sum;
+  __syncthreads();
+  if (y || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < kReduceRows; ++i) sum += s[i][x];
+  dtable[(size_t)(c % buckets) * heads + c / buckets] = sum;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+int tiles32(int x) { return (x + kTile - 1) / kTile; }
+// At most ceil(T / 128) + (non-empty segments) groups, one more where they begin at even tokens.
+size_t groups_most(int total, int batch) {
+  return (size_t)(total + kGroupTok - 1) / kGroupTok + (size_t)std::min(batch, total) + 1;
+}
+
+struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, line, top, ranges, knorm, rows, part, total; };
+Layout layout(int batch, int total_q, int total_k, int heads, int buckets, int reach, int dtype, bool backward) {
+  Layout w{};
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += up256(bytes);
+    return at;
+  };
+  const int stride = 2 * (reach + kRelPad) + 1;
+  const size_t gq = groups_most(total_q, batch), gk = groups_most(total_k, batch);
+  w.counts = take(8);
+  w.plan_q = take(gq * sizeof(int4));
+  w.shift_q = take(gq * sizeof(int));
+  w.line = take((size_t)heads * stride * sizeof(float));
+  w.top = take(heads * sizeof(float));
+  w.ranges = take(buckets * sizeof(int2));
+  if (backward) {
+    w.plan_k = take(gk * sizeof(int4));
+    w.shift_k = take(gk * sizeof(int));
+    w.rows = take((size_t)heads * tiles32(total_q) * kTile * sizeof(float2));
+    w.part = take(gq * heads * buckets * sizeof(float));
+  } else if (dtype == ESA_BF16) {
+    w.knorm = take((size_t)heads * tiles32(total_k) * sizeof(float));
+  }
+  w.total = off;
+  return w;
+}
+
+int check(int batch, int total_q, int total_k, int heads, int head_dim, int dtype, int buckets, const int* starts,
+          int side) {
+  if (head_dim != 16 && head_dim != 24 && head_dim != 32 && head_dim != 64) return ESA_ERR_HEAD_DIM;
+  if (dtype != ESA_BF16 && dtype != ESA_F32) return ESA_ERR_DTYPE;
+  // token offsets and distances (a query offset of up to 2^30 among them) stay within 32 bits
+  if (batch < 1 || heads < 1 || total_q < 0 || total_k < 0 || total_q >= 1 << 29 || total_k >= 1 << 29) return ESA_ERR_SHAPE;
+  if ((groups_most(std::max(total_q, total_k), batch) + 1) * (size_t)heads >= (size_t)1 << 31) return ESA_ERR_SHAPE;
+  if (!starts) return ESA_ERR_NULL;
+  if (buckets < 1 || buckets > kRelMaxBuckets || side < 1 || side > kRelMaxBuckets / 2 ||
+      (side != buckets && 2 * side != buckets))
+    return ESA_ERR_SHAPE;
+  if (starts[0] != 0 || starts[side - 1] > kRelMaxReach) return ESA_ERR_SHAPE;
+  for (int i = 1; i < side; ++i)
+    if (starts[i] < starts[i - 1]) return ESA_ERR_SHAPE;
+  return ESA_OK;
+}
+
+bool off_boundary(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// From 1 on: distance 0 is in neither constant end of the line.
+int reach_of(const int* starts, int side) { return std::max(1, starts[side - 1]); }
+
+void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buckets, const int* starts, int side,
+          const int* q_start, const DenseAttnCall& c, int dtype, bool backward, RelPass& r, RelPrep& p) {
+  auto at = [&](size_t off) { return ws + off; };
+  RelBias& b = r.bias;
+  b.reach = reach_of(starts, side);
+  b.stride = 2 * (b.reach + kRelPad) + 1;
+  b.buckets = buckets;
+  b.far_lo = side - 1;
+  b.far_hi = buckets == side ? 0 : buckets - 1;
+  p.line = reinterpret_cast<float*>(at(w.line)); p.top = reinterpret_cast<float*>(at(w.top));
+  p.ranges = reinterpret_cast<int2*>(at(w.ranges));
+  b.line = p.line; b.top = p.top; b.ranges = p.ranges;
+  b.part = backward ? reinterpret_cast<float*>(at(w.part)) : nullptr;
+  r.plan_q = reinterpret_cast<int4*>(at(w.plan_q));
+  r.shift_q = reinterpret_cast<int*>(at(w.shift_q));
+  r.count_q = reinterpret_cast<int*>(at(w.counts));
+  r.count_k = r.count_q + 1;
+  r.tq_pad = tiles32(c.total_q) * kTile;
+  if (backward) {
+    r.plan_k = reinterpret_cast<int4*>(at(w.plan_k));
+    r.shift_k = reinterpret_cast<int*>(at(w.shift_k));
+    r.rows = reinterpret_cast<float2*>(at(w.rows));
+  } else if (dtype == ESA_BF16) {
+    r.knorm = reinterpret_cast<float*>(at(w.knorm));
+    r.tk_tiles = tiles32(c.total_k);
+  }
+  p.cu_q = c.cu_q; p.cu_k = c.cu_k; p.q_start = q_start; p.nseg = c.nseg;
+  p.total_q = c.total_q; p.total_k = c.total_k; p.heads = c.heads;
+  p.row16 = c.heads * c.head_dim * (dtype == ESA_F32 ? 4 : 2) / 16;
+  p.table = table; p.table_dtype = table_dtype;
+  std::copy(starts, starts + side, p.starts);
+  p.side = side; p.two_sided = side != buckets;
+  p.zero_q = static_cast<uint4*>(backward ? c.dq : c.out);
+  p.zero_k = static_cast<uint4*>(c.dk); p.zero_v = static_cast<uint4*>(c.dv);
+  p.lse = backward ? nullptr : c.lse;
+  p.backward = backward;
+  p.key_pairs = backward && c.dropout && dtype == ESA_BF16;   // the bf16 dK/dV pass shares its hashes by key pairs
+}
+
+}  // namespace
+
+extern "C" {
+
+int esa_rel_attn_workspace_size(int batch, int total_q, int total_k, int heads, int head_dim, int dtype, int num_buckets,
+                                const int* bucket_starts, int num_starts, int backward, size_t* bytes) {
+  if (!bytes) return ESA_ERR_NULL;
+  const int rc = check(batch, total_q, total_k, heads, head_dim, dtype, num_buckets, bucket_starts, num_starts);
+  if (rc) return rc;
+  *bytes = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, backward != 0).total;
+  return ESA_OK;
+}
+
+int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, int table_dtype, int num_buckets,
+                     const int* bucket_starts, int num_starts, const int* q_start, const int* cu_seqlens_q,
+                     const int* cu_seqlens_k, int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
+                     float softmax_scale, float dropout_p, unsigned long long dropout_seed, void* out, float* softmax_lse,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(batch, total_q, total_k, heads, head_dim, dtype, num_buckets, bucket_starts, num_starts);
+  if (rc) return rc;
+  if (table_dtype != ESA_BF16 && table_dtype != ESA_F32) return ESA_ERR_DTYPE;
+  if (!(dropout_p >= 0.f && dropout_p < 1.f)) return ESA_ERR_DROPOUT;
+  if (!(softmax_scale > 0.f && softmax_scale <= 3.0e38f)) return ESA_ERR_SHAPE;
+  if (total_q == 0) return ESA_OK;
+  if (!table || !cu_seqlens_q || !cu_seqlens_k || !workspace || !q || !out || !softmax_lse || (total_k > 0 && (!k || !v)))
+    return ESA_ERR_NULL;
+  if (off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(workspace))
+    return ESA_ERR_ALIGN;
+  const Layout w = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, false);
+  if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
+  DenseAttnCall c{};
+  c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;
+  c.total_q = total_q; c.total_k = total_k; c.heads = heads; c.head_dim = head_dim; c.scale = softmax_scale;
+  c.out = out; c.lse = softmax_lse;
+  c.drop = make_dropout(dropout_p, dropout_seed, heads); c.dropout = dropout_p > 0.f;
+  RelPass r{};
+  RelPrep p{};
+  fill(w, static_cast<char*>(workspace), table, table_dtype, num_buckets, bucket_starts, num_starts, q_start, c, dtype, false, r,
+       p);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return dtype == ESA_BF16 ? wide_rel_fwd(c, r, p, st) : f32_rel_fwd(c, r, p, st);
+}
+
+int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                     const float* softmax_lse, const void* table, int table_dtype, int num_buckets,
+                     const int* bucket_starts, int num_starts, const int* q_start, const int* cu_seqlens_q,
+                     const int* cu_seqlens_k, int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
+                     float softmax_scale, float dropout_p, unsigned long long dropout_seed, void* dq, void* dk, void* dv,
+                     float* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(batch, total_q, total_k, heads, head_dim, dtype, num_buckets, bucket_starts, num_starts);
+  if (rc) return rc;
+  if (table_dtype != ESA_BF16 && table_dtype != ESA_F32) return ESA_ERR_DTYPE;
+  if (!(dropout_p >= 0.f && dropout_p < 1.f)) return ESA_ERR_DROPOUT;
+  if (!(softmax_scale > 0.f && softmax_scale <= 3.0e38f)) return ESA_ERR_SHAPE;
+  if (!table || !dtable || !cu_seqlens_q || !cu_seqlens_k || !workspace ||
+      (total_q > 0 && (!dout || !q || !out || !softmax_lse || !dq)) || (total_k > 0 && (!k || !v || !dk || !dv)))
+    return ESA_ERR_NULL;
+  if (off_boundary(dout) || off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(dq) ||
+      off_boundary(dk) || off_boundary(dv) || off_boundary(workspace))
+    return ESA_ERR_ALIGN;
+  const Layout w = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, true);
+  if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
+  DenseAttnCall c{};
+  c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;
+  c.total_q = total_q; c.total_k = total_k; c.heads = heads; c.head_dim = head_dim; c.scale = softmax_scale;
+  c.out_in = out; c.dout = dout; c.lse_in = softmax_lse; c.dq = dq; c.dk = dk; c.dv = dv;
+  c.drop = make_dropout(dropout_p, dropout_seed, heads); c.dropout = dropout_p > 0.f;
+  RelPass r{};
+  RelPrep p{};
+  fill(w, static_cast<char*>(workspace), table, table_dtype, num_buckets, bucket_starts, num_starts, q_start, c, dtype, true, r, p);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  rc = dtype == ESA_BF16 ? wide_rel_bwd(c, r, p, st) : f32_rel_bwd(c, r, p, st);
+  if (rc) return rc;
+  ESA_TIMED(esa_profile::kColumnSum, st,
+            hipLaunchKernelGGL(rel_reduce_kernel, dim3((unsigned)((heads * num_buckets + kReduceCols - 1) / kReduceCols)),
+                               dim3(kReduceCols * kReduceRows), 0, st, r.bias.part, r.count_q, heads, num_buckets, dtable));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+}  // extern "C"

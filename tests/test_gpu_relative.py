@@ -1,0 +1,304 @@
+"""Varlen attention with a learned bias by relative position against the formula in 64 bits: head dims, types, lengths
+from none to long, segments without keys, query offsets, one- and two-sided buckets, -inf entries, dropout, gradients.
+
+Tolerances.  bf16 calls: the inputs are exact in 64 bits; P and dS enter their products rounded to bf16 (2^-8 each half
+a step at most 2^-9 relative) and the result is rounded once more, so an output's error is at most 2^-8 of the largest
+sum of absolute terms; the norm-wise bars of 6e-3 leave what independent roundings (2^-9 / sqrt 3 each, three of them)
+do not use.  The backward takes D = sum(dO O) from the rounded O, one more of the same size.  The table's gradient sums dS,
+whose terms cancel (over all of a row's keys to nothing), and roundings are relative to the terms: D's error e, about
+2^-9 sqrt(sum of (P dP)^2) for a row, enters a bucket's sum as e times the row's P in the bucket, at most 2^-9 of
+sqrt(sum dS^2) where the bucket holds the whole row.  Its error is therefore held against the larger of its norm and the
+norm of the buckets' sqrt(sum dS^2), the size such a sum has when its terms do not happen to cancel.  float32: products and sums
+in 24 bits, exponentials within a few units of 2^-24 times |score| (up to about 20 here): 1e-5 norm-wise, as for the
+other float32 attention kernels."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mind_amd import _lib
+from mind_amd.esa.relative import bucket_starts, relative_attention
+from oracle.dropout import keep_mask, params
+from tests._util import cu_from_lengths, seeded_normal
+
+pytestmark = pytest.mark.gpu
+
+
+def buckets_of(d, num_buckets, max_distance, bidirectional):
+    starts = torch.tensor(bucket_starts(num_buckets, max_distance, bidirectional))
+    far = d.abs() if bidirectional else (-d).clamp(min=0)
+    b = torch.searchsorted(starts, far.contiguous(), right=True) - 1
+    return b + (d > 0).long() * len(starts) if bidirectional else b
+
+
+def oracle(q, k, v, bias, lens_q, lens_k, max_distance=128, bidirectional=True, starts=None, g=None, scale=None, keep=None):
+    """(out, lse, dq, dk, dv, dbias, sqrt(sum dS^2) by bucket) in 64 bits on the CPU; keep: [H, Tq, Tk] scaled mask."""
+    q, k, v, bias = (x.detach().double().cpu() for x in (q, k, v, bias))
+    h, hd, nb = q.shape[1], q.shape[2], bias.shape[0]
+    scale = 1 / math.sqrt(hd) if scale is None else scale
+    out, dq, dk, dv = (torch.zeros_like(x) for x in (q, q, k, v))
+    lse = torch.full((h, q.shape[0]), -math.inf, dtype=torch.float64)
+    db, sq, qs, ks = torch.zeros_like(bias), torch.zeros_like(bias), 0, 0
+    for s, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        a, b = slice(qs, qs + lq), slice(ks, ks + lk)
+        qs, ks = qs + lq, ks + lk
+        if lq == 0 or lk == 0:
+            continue
+        d = torch.arange(lk)[None, :] - torch.arange(lq)[:, None] - (0 if starts is None else starts[s])
+        bk = buckets_of(d, nb, max_distance, bidirectional)
+        x = torch.einsum("ihd,jhd->hij", q[a], k[b]) * scale + bias[bk].permute(2, 0, 1)
+        lse[:, a] = torch.logsumexp(x, 2)
+        p = torch.exp(x - lse[:, a, None])
+        p[torch.isneginf(lse[:, a])] = 0
+        z = 1.0 if keep is None else keep[:, a, b]
+        out[a] = torch.einsum("hij,jhd->ihd", p * z, v[b])
+        if g is None:
+            continue
+        gx = g.detach().double().cpu()[a]
+        dp = torch.einsum("ihd,jhd->hij", gx, v[b]) * z
+        ds = p * (dp - (p * dp).sum(2, keepdim=True))
+        dq[a] = torch.einsum("hij,jhd->ihd", ds, k[b]) * scale
+        dk[b] = torch.einsum("hij,ihd->jhd", ds, q[a]) * scale
+        dv[b] = torch.einsum("hij,ihd->jhd", p * z, gx)
+        db.index_add_(0, bk.reshape(-1), ds.permute(1, 2, 0).reshape(-1, h))
+        sq.index_add_(0, bk.reshape(-1), ds.square().permute(1, 2, 0).reshape(-1, h))
+    return out, lse, dq, dk, dv, db, sq.sqrt()
+
+
+def case(device, dtype, h, hd, lens_q, lens_k=None, buckets=32, seed=0, table=torch.float32, extra=0):
+    same = lens_k is None
+    lens_k = lens_q if same else lens_k
+    tq, tk = sum(lens_q) + extra, sum(lens_k) + extra
+    q, k, v, g = (seeded_normal((t, h, hd), seed + i, dtype).to(device) for i, t in enumerate((tq, tk, tk, tq)))
+    bias = seeded_normal((buckets, h), seed + 9, torch.float32).to(table).to(device)
+    cu_q = torch.as_tensor(cu_from_lengths(lens_q)).to(device)
+    cu_k = cu_q if same else torch.as_tensor(cu_from_lengths(lens_k)).to(device)
+    return q, k, v, g, bias, cu_q, cu_k
+
+
+def scaled_keep(p, seed, h, tq, tk):
+    return torch.as_tensor(keep_mask(p, seed, h, np.arange(tq), np.arange(tk))).double() * params(p, seed)[3]
+
+
+def rel_err(got, ref):
+    got, ref = got.detach().double().cpu(), ref.double()
+    assert torch.isfinite(got).all()
+    return float((got - ref).norm()) / max(float(ref.norm()), 1e-30) if ref.norm() > 0 else float(got.abs().sum())
+
+
+def check(device, dtype, h, hd, lens_q, lens_k=None, buckets=32, max_distance=128, bidirectional=True, starts=None, seed=0,
+          table=torch.float32, extra=0, dropout=0.0, bias=None):
+    q, k, v, g, b, cu_q, cu_k = case(device, dtype, h, hd, lens_q, lens_k, buckets, seed, table, extra)
+    if bias is not None:
+        b = bias(b)
+    q0 = None if starts is None else torch.tensor(starts, dtype=torch.int32, device=device)
+    leaves = [x.requires_grad_(True) for x in (q, k, v, b)]
+    out, lse = relative_attention(*leaves, cu_q, cu_k, max_distance=max_distance, bidirectional=bidirectional, q_start=q0,
+                                  return_lse=True, dropout_p=dropout, dropout_seed=77)
+    grads = torch.autograd.grad(out, leaves, g)
+    keep = None
+    if dropout:
+        keep = scaled_keep(dropout, 77, h, q.shape[0], k.shape[0])
+    ref = oracle(q, k, v, b, lens_q, lens_k or lens_q, max_distance, bidirectional, starts, g, keep=keep)
+    bar = 1e-5 if dtype == torch.float32 else 6e-3
+    assert grads[3].dtype == table
+    errs = [rel_err(x, r) for x, r in zip((out, *grads), (ref[0], *ref[2:5]))]
+    size = max(float(ref[5].norm()), float(ref[6].norm()))
+    errs.append(float((grads[3].detach().double().cpu() - ref[5]).norm()) / size if size else float(grads[3].abs().max()))
+    assert all(e <= bar for e in errs[:4]), errs
+    assert errs[4] <= (max(bar, 4e-3) if table == torch.bfloat16 else bar), errs
+    assert torch.isfinite(grads[3]).all()
+    dead = torch.isneginf(ref[1])
+    assert torch.equal(torch.isneginf(lse.cpu()), dead)
+    # the lse of a bf16 call is of exact products too; its row sum adds probabilities rounded to bf16
+    off = (lse.cpu().double() - ref[1])[~dead].abs()
+    assert not off.numel() or float(off.max()) <= (2.0 ** -8 if dtype == torch.bfloat16 else 2e-5)
+    return q, k, v, b, out, grads
+
+
+LENGTHS = ([1], [2, 1, 31], [33, 0, 64, 65], [127, 128, 129], [1, 300, 17], [700])
+
+
+@pytest.mark.parametrize("hd", [16, 24, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens", LENGTHS, ids=str)
+def test_self_attention(device, dtype, hd, lens):
+    check(device, dtype, 3, hd, lens)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 64), (torch.float32, 16), (torch.float32, 64)])
+@pytest.mark.parametrize("buckets,distance,two", [(32, 128, False), (4, 2, True), (8, 20, True), (2, 900, False),
+                                                  (64, 512, True), (256, 768, True), (128, 700, False), (12, 7, True)])
+def test_buckets(device, dtype, hd, buckets, distance, two):
+    check(device, dtype, 2, hd, [450, 5, 901], buckets=buckets, max_distance=distance, bidirectional=two, seed=3)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 32), (torch.float32, 16), (torch.float32, 64)])
+@pytest.mark.parametrize("lens_q,lens_k,starts", [
+    ([1, 1, 1], [500, 1, 77], [499, 0, 76]), ([3, 0, 40], [200, 30, 0], None), ([130, 5], [70, 300], [-40, 295]),
+    ([64, 64], [64, 64], [2 ** 31 - 1, -2 ** 31]), ([0, 0], [5, 40], None), ([33], [257], [1000])], ids=str)
+def test_query_chunks(device, dtype, hd, lens_q, lens_k, starts):
+    check(device, dtype, 2, hd, lens_q, lens_k, starts=starts, seed=5)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 24), (torch.float32, 32)])
+def test_dropout(device, dtype, hd):
+    check(device, dtype, 2, hd, [33, 150, 1, 200], dropout=0.25, seed=7)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_bf16_table_and_tokens_in_no_segment(device, dtype):
+    q, k, v, b, out, grads = check(device, dtype, 4, 16, [50, 200], table=torch.bfloat16, extra=37, seed=11)
+    assert not out[250:].any() and not any(x[250:].any() for x in grads[:3])
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.float32, 16), (torch.bfloat16, 64)])
+def test_masking_entries(device, dtype, hd):
+    """-inf entries leave their pairs out, also where that leaves a row empty; entries of the type's lowest value leave a
+    row of nothing else its plain softmax; a large spread takes the running maximum."""
+    lens = [300, 40]
+
+    def ahead(b):   # keys after the query left out, and in head 1 everything
+        b = b.clone()
+        b[16:] = -math.inf
+        b[:, 1] = -math.inf
+        return b
+
+    def lowest(b):
+        b = b.clone()
+        b[:, 0] = torch.finfo(torch.float32).min
+        return b
+
+    def wide(b):
+        return b * 40
+    check(device, dtype, 3, hd, lens, bias=ahead, seed=13)
+    check(device, dtype, 3, hd, lens, bias=wide, seed=15)
+    q, k, v, g, b, cu, _ = case(device, dtype, 3, hd, lens, seed=17)
+    got = relative_attention(q, k, v, lowest(b), cu, cu)
+    plain = b.clone()
+    plain[:, 0] = 0
+    ref = oracle(q, k, v, plain, lens, lens)[0]
+    # |bias| log2(e) is 14,427, one unit of whose last place is 2^-10: the exponents are off by at most that much
+    assert rel_err(got, ref) <= 6e-3
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 32), (torch.float32, 16)])
+def test_other_segments_values_do_not_leak(device, dtype, hd):
+    """A graph with infinities and NaN leaves its neighbours' outputs and gradients as they are: the same bits in float32;
+    in bf16 the forward's reference point (fixed or running maximum) goes by key norms of 32-token tiles, which may hold
+    a neighbour's, so both results are within the bar of the formula, and of each other within twice that."""
+    lens = [45, 70, 33]
+    q, k, v, g, b, cu, _ = case(device, dtype, 2, hd, lens, seed=19)
+
+    def run(q, k, v, g):
+        leaves = [x.detach().clone().requires_grad_(True) for x in (q, k, v)]
+        out = relative_attention(*leaves, b, cu, cu)
+        return (out, *torch.autograd.grad(out, leaves, g))
+    good = run(q, k, v, g)
+    bad = [x.clone() for x in (q, k, v, g)]
+    for x, bad_value in zip(bad, (math.nan, math.inf, math.nan, -math.inf)):
+        x[45:115] = bad_value
+    for x, y in zip(good, run(*bad)):
+        for s in (slice(0, 45), slice(115, None)):
+            assert torch.equal(x[s], y[s]) if dtype == torch.float32 else rel_err(y[s], x[s].detach().cpu()) <= 1.2e-2
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.float32, 32)])
+def test_gradients_against_differences(device, dtype, hd):
+    """The table's and v's gradients against central differences of the 64-bit formula."""
+    lens = [60, 5]
+    q, k, v, g, b, cu, _ = case(device, dtype, 2, hd, lens, seed=23)
+    vv, bb = v.detach().requires_grad_(True), b.detach().requires_grad_(True)
+    out = relative_attention(q, k, vv, bb, cu, cu)
+    dv, db = torch.autograd.grad(out, (vv, bb), g)
+    gen, eps = torch.Generator().manual_seed(5), 1e-4
+    tb, tv = torch.randn(b.shape, generator=gen).double(), torch.randn(v.shape, generator=gen).double()
+
+    def f(e, f_):
+        o = oracle(q, k, v.cpu().double() + f_ * tv, b.cpu().double() + e * tb, lens, lens)[0]
+        return float((o * g.cpu().double()).sum())
+    bar = 6e-3 if dtype == torch.bfloat16 else 2e-5   # a gradient off by bar * |gradient| moves its product with t by this
+    for grad, t, diff in ((db, tb, f(eps, 0) - f(-eps, 0)), (dv, tv, f(0, eps) - f(0, -eps))):
+        diff /= 2 * eps
+        assert abs(float((grad.cpu().double() * t).sum()) - diff) <= bar * float(grad.double().norm().cpu() * t.norm())
+
+
+def test_same_bits_twice_and_on_another_stream(device):
+    q, k, v, g, b, cu, _ = case(device, torch.bfloat16, 8, 16, [700, 33, 512], seed=29)
+
+    def run():
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v, b)]
+        out = relative_attention(*leaves, cu, cu)
+        return (out, *torch.autograd.grad(out, leaves, g))
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+
+
+def test_captured_and_replayed(device):
+    """Forward and backward in one graph, replayed with other inputs between eager calls."""
+    q, k, v, g, b, cu, _ = case(device, torch.bfloat16, 4, 16, [200, 77], seed=31)
+
+    def step():
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v, b)]
+        out = relative_attention(*leaves, cu, cu)
+        return (out, *torch.autograd.grad(out, leaves, g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (1, 2, 3):
+        for x in (q, k, v, g, b):
+            x.copy_(seeded_normal(tuple(x.shape), 100 * seed + x.shape[0], torch.float32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(held, step()))
+
+
+def test_longest_line_and_many_buckets(device):
+    """The largest reach and the largest table, whose sums need most of a CU's LDS."""
+    check(device, torch.float32, 1, 64, [1800], buckets=256, max_distance=768, seed=37)
+    check(device, torch.bfloat16, 2, 64, [1800, 3], buckets=256, max_distance=768, seed=37)
+
+
+def test_larger_than_one_group(device):
+    check(device, torch.bfloat16, 16, 16, [900, 1500, 64, 3], seed=41)
+    check(device, torch.float32, 8, 16, [340] * 5, seed=43)
+
+
+def test_no_tokens(device):
+    for lens_q, lens_k in (([0], [0]), ([0], [9]), ([9], [0])):
+        check(device, torch.bfloat16, 2, 16, lens_q, lens_k)
+        check(device, torch.float32, 2, 16, lens_q, lens_k)
+
+
+def test_output_gradient_off_a_boundary_and_strided(device):
+    q, k, v, g, b, cu, _ = case(device, torch.bfloat16, 2, 16, [50, 20], seed=47)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, b)]
+    out = relative_attention(*leaves, cu, cu)
+    want = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    off = torch.empty(g.numel() + 1, dtype=g.dtype, device=device)[1:].view(g.shape).copy_(g)
+    turned = g.transpose(0, 1).contiguous().transpose(0, 1)
+    for other in (off, turned):
+        assert all(torch.equal(x, y) for x, y in zip(want, torch.autograd.grad(out, leaves, other, retain_graph=True)))
+
+
+def test_refused_on_the_device(device):
+    q, k, v, g, b, cu, _ = case(device, torch.bfloat16, 2, 16, [8])
+    with pytest.raises(_lib.EsaError, match="ALIGN"):
+        flat = torch.empty(q.numel() + 1, dtype=q.dtype, device=device)
+        relative_attention(flat[1:].view(q.shape).copy_(q), k, v, b, cu, cu)
+    leaf = q.detach().requires_grad_(True)
+    out = relative_attention(leaf, k, v, b, cu, cu)
+    (grad,) = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.float().sum().backward()
