@@ -568,6 +568,60 @@ ESA_API int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, con
                    size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* RMS norm of every query and key head row with the rotation of positions   */
+/* in the same pass (no counterpart in the reference).                       */
+/*                                                                           */
+/* q [total, heads_q, head_dim] and k [total, heads_k, head_dim] of `dtype`,  */
+/* head_dim 16, 24, 32 or 64, rows of head_dim consecutive elements; strides: */
+/* host array {q token, q head, k token, k head} in elements, multiples of    */
+/* 16 bytes.  heads_k 0: queries alone.  y = x w / sqrt(mean(x^2) + eps), wq  */
+/* / wk fp32 [head_dim] or null (ones).  The first rotary_dim dims (a         */
+/* multiple of 8; 0: none) in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1)  */
+/* where interleaved, are turned by positions[token] * frequencies[i]         */
+/* radians, worked out in 64 bits: positions of positions_bytes 4 or 8, any   */
+/* value; frequencies fp64 [rotary_dim / 2].  Outputs [total, heads,          */
+/* head_dim] contiguous, rounded once.                                        */
+/*                                                                           */
+/* _bwd: gq, gk and dq, dk contiguous; dwq, dwk fp32 or null, in a fixed      */
+/* order (deterministic), of q's and k's rows; a null workspace if both are   */
+/* null.  heads_q, heads_k up to 2048; pointers 16-byte aligned.              */
+/* ------------------------------------------------------------------------ */
+ESA_API int esa_qk_norm_fwd(const void* q, const void* k, const long long* strides, int total,
+                   int heads_q, int heads_k, int head_dim, int dtype, const float* wq,
+                   const float* wk, const void* positions, int positions_bytes,
+                   const double* frequencies, int rotary_dim, int interleaved, float eps,
+                   void* q_out, void* k_out, void* stream);
+ESA_API int esa_qk_norm_bwd_workspace_size(int total, int head_dim, size_t* bytes);
+ESA_API int esa_qk_norm_bwd(const void* gq, const void* gk, const void* q, const void* k,
+                   const long long* strides, int total, int heads_q, int heads_k, int head_dim,
+                   int dtype, const float* wq, const float* wk, const void* positions,
+                   int positions_bytes, const double* frequencies, int rotary_dim,
+                   int interleaved, float eps, void* dq, void* dk, float* dwq, float* dwk,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* The norm over the values of many tensors together, and the tensors times  */
+/* the factor that clips it: the gradient norm that the reference logs with   */
+/* one host read per parameter (core/pretraining_model.py:606-612) and the    */
+/* clipping of its trainer.                                                   */
+/*                                                                           */
+/* n tensors by host arrays of device pointers, element counts and dtypes     */
+/* (ESA_F32 or ESA_BF16), each contiguous, at any element alignment.          */
+/* esa_grad_norm: *norm (device fp32) = sqrt(sum of squares) (infinity 0) or  */
+/* the largest absolute value (infinity 1, a NaN staying one); squares are    */
+/* summed in fp64 in a fixed order.  esa_grad_clip: out_i = in_i *            */
+/* min(1, max_norm / (*norm + 1e-6)) (a NaN norm gives NaN), rounded once;    */
+/* out_i may be in_i; out dtypes in_i's or ESA_F32.  No tensors: norm 0.      */
+/* ------------------------------------------------------------------------ */
+ESA_API int esa_grad_norm_workspace_size(int n, const long long* counts, size_t* bytes);
+ESA_API int esa_grad_norm(int n, const void* const* in, const long long* counts, const int* dtypes,
+                   int infinity, float* norm, void* workspace, size_t workspace_bytes,
+                   void* stream);
+ESA_API int esa_grad_clip(int n, const void* const* in, void* const* out, const long long* counts,
+                   const int* in_dtypes, const int* out_dtypes, float max_norm,
+                   const float* norm, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Profiling hook (no counterpart in the reference; used by the benchmark).  */
 /* While enabled, every kernel launch of the entry points above is           */
 /* bracketed by hipEvents on its stream.  esa_profile_collect waits for the  */
@@ -575,7 +629,7 @@ ESA_API int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, con
 /* launch count per kernel id (capacity >= ESA_PROFILE_KERNELS) and clears   */
 /* the record.  Not for concurrent use from several threads.                 */
 /* ------------------------------------------------------------------------ */
-#define ESA_PROFILE_KERNELS 25
+#define ESA_PROFILE_KERNELS 29
 ESA_API int esa_profile_enable(int on);
 ESA_API int esa_profile_collect(float* total_ms, int* launches, int capacity);
 ESA_API const char* esa_profile_kernel_name(int kernel);

@@ -128,6 +128,21 @@ _PROTOS = {
     "esa_rel_attn_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int, _vp,
                                   _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp,
                                   _vp, _vp, _vp, _c_sz, _vp]),
+    # q k strides[4] total hq hk hd dtype | wq wk positions bytes frequencies rotary interleaved eps | q_out k_out stream
+    "esa_qk_norm_fwd": (_c_int, [_vp, _vp, ctypes.POINTER(ctypes.c_longlong), _c_int, _c_int, _c_int, _c_int, _c_int, _vp,
+                                 _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_f, _vp, _vp, _vp]),
+    "esa_qk_norm_bwd_workspace_size": (_c_int, [_c_int, _c_int, ctypes.POINTER(_c_sz)]),
+    # gq gk | as the forward up to eps | dq dk dwq dwk ws bytes stream
+    "esa_qk_norm_bwd": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_longlong), _c_int, _c_int, _c_int, _c_int,
+                                 _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_f, _vp, _vp, _vp, _vp, _vp, _c_sz,
+                                 _vp]),
+    "esa_grad_norm_workspace_size": (_c_int, [_c_int, ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(_c_sz)]),
+    # n in[] counts[] dtypes[] infinity | norm ws bytes stream
+    "esa_grad_norm": (_c_int, [_c_int, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(_c_int),
+                               _c_int, _vp, _vp, _c_sz, _vp]),
+    # n in[] out[] counts[] in_dtypes[] out_dtypes[] | max_norm norm stream
+    "esa_grad_clip": (_c_int, [_c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_longlong),
+                               ctypes.POINTER(_c_int), ctypes.POINTER(_c_int), _c_f, _vp, _vp]),
     "esa_mab_residual_fwd": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _vp, _vp]),
     "esa_mab_residual_bwd": (_c_int, [_vp, _vp, _c_i64, _c_int, _vp, _vp, _vp]),
     "esa_profile_enable": (_c_int, [_c_int]),
@@ -135,7 +150,7 @@ _PROTOS = {
     "esa_profile_kernel_name": (ctypes.c_char_p, [_c_int]),
 }
 
-PROFILE_KERNELS = 25
+PROFILE_KERNELS = 29
 
 _lock = threading.Lock()
 _lib = None

@@ -32,6 +32,10 @@ enum Kernel : int {
   kLinearF32,         // fp32 Linear layers of the blocks
   kLinearGemm,        // the blocks' Linears with their epilogues, and their input gradients
   kWeightGrad,        // weight and bias gradients of the blocks' Linear layers
+  kQkNormFwd,         // query and key norms with the rotation
+  kQkNormBwd,
+  kGradNorm,          // global gradient norm: sums of squares
+  kGradClip,          // the clipped gradients
   kNumKernels
 };
 

@@ -1,0 +1,145 @@
+"""Norms of queries and keys per head with the rotation of positions in the same pass (esa_qk_norm_fwd / _bwd).
+
+``qk_norm_rotary`` takes projected query and key rows to what attention over
+ordered tokens uses: each head's row divided by its root mean square, scaled
+by weights shared by the heads, and its first dimensions rotated in pairs by
+the token's position.  The reference has no counterpart: its layers see a set.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .attention import HEAD_DIMS
+from .eager import call
+from .layer_norm import f32_values
+from .linear import on_boundary
+
+_CODES = {torch.float32: _lib.ESA_F32, torch.bfloat16: _lib.ESA_BF16}
+MAX_HEADS = 2048
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The radians per position of each pair, base ** (-2 i / rotary_dim), float64 [rotary_dim / 2]."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive (got {rotary_dim})")
+    return float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x, or its copy where its rows are not 16-byte aligned runs."""
+    size = x.element_size()
+    if (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(q, k):
+    return (ctypes.c_longlong * 4)(q.stride(0), q.stride(1), *((0, 0) if k is None else (k.stride(0), k.stride(1))))
+
+
+def _common(q, k, wq, wk, positions, frequencies, interleaved, eps):
+    """The C ABI's arguments from `total` to eps."""
+    turned = frequencies is not None
+    return (q.shape[0], q.shape[1], 0 if k is None else k.shape[1], q.shape[2], _CODES[q.dtype], _lib.ptr(wq), _lib.ptr(wk),
+            _lib.ptr(positions), positions.element_size() if turned else 0, _lib.ptr(frequencies),
+            2 * frequencies.numel() if turned else 0, int(interleaved), eps)
+
+
+class _QkNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+        ctx.weight_dtypes = [None if w is None else w.dtype for w in (q_weight, k_weight)]
+        q, k = _rows(q), None if k is None else _rows(k)
+        wq, wk = f32_values(q_weight), f32_values(k_weight)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        with _lib.on_device(q):
+            _lib.check(_lib.load().esa_qk_norm_fwd(
+                q.data_ptr(), _lib.ptr(k), _strides(q, k), *_common(q, k, wq, wk, positions, frequencies, interleaved, eps),
+                q_out.data_ptr(), _lib.ptr(k_out), _lib.stream_of(q)), "esa_qk_norm_fwd")
+        ctx.save_for_backward(q, k, wq, wk, positions, frequencies)
+        ctx.meta = (eps, interleaved)
+        return (q_out, k_out) if k is not None else q_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk=None):
+        q, k, wq, wk, positions, frequencies = ctx.saved_tensors
+        eps, interleaved = ctx.meta
+        gq, gk = on_boundary(gq.contiguous()), None if k is None else on_boundary(gk.contiguous())
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dws = [torch.empty(q.shape[2], dtype=torch.float32, device=q.device) if n else None for n in ctx.needs_input_grad[2:4]]
+        lib, ws = _lib.load(), None
+        with _lib.on_device(q):
+            if any(w is not None for w in dws):
+                n = ctypes.c_size_t(0)
+                _lib.check(lib.esa_qk_norm_bwd_workspace_size(q.shape[0], q.shape[2], ctypes.byref(n)),
+                           "esa_qk_norm_bwd_workspace_size")
+                ws = torch.empty(max(int(n.value), 256), dtype=torch.uint8, device=q.device)
+            _lib.check(lib.esa_qk_norm_bwd(
+                gq.data_ptr(), _lib.ptr(gk), q.data_ptr(), _lib.ptr(k), _strides(q, k),
+                *_common(q, k, wq, wk, positions, frequencies, interleaved, eps), dq.data_ptr(), _lib.ptr(dk),
+                _lib.ptr(dws[0]), _lib.ptr(dws[1]), _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q)),
+                "esa_qk_norm_bwd")
+        dwq, dwk = (w if w is None else w.to(t) for w, t in zip(dws, ctx.weight_dtypes))
+        return dq, dk, dwq, dwk, None, None, None, None
+
+
+def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
+    if x.dtype not in _CODES:
+        raise TypeError(f"{name} must be float32 or bfloat16 (got {x.dtype})")
+    if x.dim() != 3 or x.shape[2] not in HEAD_DIMS or not 1 <= x.shape[1] <= MAX_HEADS:
+        raise ValueError(f"{name} must be [total, heads, head_dim] with 1 to {MAX_HEADS} heads and head_dim in {HEAD_DIMS} "
+                         f"(got {tuple(x.shape)})")
+    if like is not None and (x.dtype != like.dtype or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2]):
+        raise ValueError(f"{name} must have the tokens, head_dim and dtype of q (got {tuple(x.shape)}, {x.dtype})")
+
+
+def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, frequencies=None, eps=1e-6, interleaved=False):
+    """(q', k') of query rows q [T, Hq, hd] and key rows k [T, Hk, hd] (k None: q' alone); hd 16, 24, 32 or 64, float32
+    or bfloat16 with float32 arithmetic, rounded once.
+
+    y = x / sqrt(mean(x ** 2) + eps) * weight over each head's row; q_weight / k_weight: [hd] or None (ones).  With
+    ``positions`` (int32 or int64 [T], any values) and ``frequencies`` (float64 [r / 2], ``rotary_frequencies``; r a
+    multiple of 8 up to hd), the first r dimensions are rotated in pairs (i, i + r / 2), or (2i, 2i + 1) with
+    ``interleaved``, by positions * frequencies[i], worked out in 64 bits (an angle is off by at most 2^-51 of itself).
+
+    q and k may be views (of one projection's output, say): rows of hd consecutive elements on 16-byte boundaries are
+    read where they are, others from a copy.  The outputs are contiguous.  Gradients reach q, k and the weights (summed
+    in float32 in a fixed order), once: they cannot be differentiated again.
+    """
+    _check_rows("q", q)
+    if k is not None:
+        _check_rows("k", k, q)
+    elif k_weight is not None:
+        raise ValueError("k_weight without k")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (q.shape[2],) or w.dtype not in _CODES):
+            raise ValueError(f"{name} must be a float32 or bfloat16 [{q.shape[2]}] (got {w.dtype}, {tuple(w.shape)})")
+    if (positions is None) != (frequencies is None):
+        raise ValueError("positions and frequencies must be given together")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or not positions.is_contiguous():
+            raise TypeError(f"positions must be a contiguous 1-D int32 or int64 tensor (got {positions.dtype}, "
+                            f"{tuple(positions.shape)})")
+        if positions.numel() != q.shape[0]:
+            raise ValueError(f"positions has {positions.numel()} entries, expected {q.shape[0]}")
+        if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+            raise TypeError(f"frequencies must be a contiguous 1-D float64 tensor (got {frequencies.dtype}, "
+                            f"{tuple(frequencies.shape)})")
+        r = 2 * frequencies.numel()
+        if r % 8 or not 8 <= r <= q.shape[2]:
+            raise ValueError(f"frequencies must rotate a multiple of 8 dimensions up to head_dim {q.shape[2]} (got {r})")
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative (got {eps})")
+    tensors = [t for t in (q, k, q_weight, k_weight, positions, frequencies) if t is not None]
+    _lib.require_gpu(*tensors)
+    _lib.require_one_device(*tensors)
+    return call(_QkNorm, q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))

@@ -1,0 +1,201 @@
+"""The gradient norm over many tensors and clipping, against 64 bits.
+
+Tolerances: squares are summed in float64, so the norm is off by one rounding to float32 (2^-24, held as 1e-7); the factor
+has three float32 roundings and a product one more (2^-22 of a value), a bf16 result its one rounding of 2^-8 besides."""
+import math
+
+import pytest
+import torch
+
+from mind_amd.esa.gradients import clip_grad_norm_, clip_gradients, grad_norm
+from tests._util import seeded_normal
+
+pytestmark = pytest.mark.gpu
+SIZES = [(1,), (3, 5), (), (8192,), (8193,), (0,), (4, 0), (300, 77), (16384, 2), (7,), (50001,)]
+
+
+def make(device, sizes, dtypes=(torch.float32,), seed=0, scale=1.0):
+    return [(seeded_normal((*s, 1), seed + i, torch.float32).view(s) * scale * 3.0 ** (i % 5)).to(dtypes[i % len(dtypes)])
+            .to(device) for i, s in enumerate(sizes)]
+
+
+def norm64(tensors):
+    return math.sqrt(math.fsum(float(t.double().square().sum()) for t in tensors))
+
+
+def close(got, want, dtype):
+    want = want.to(got.device)
+    bar = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -8 + 2.0 ** -22
+    assert bool(((got.double() - want).abs() <= bar * want.abs() + 1e-44).all())
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)], ids=str)
+@pytest.mark.parametrize("max_norm", [0.5, 1e9, 0.0])
+def test_in_place(device, dtypes, max_norm):
+    grads = make(device, SIZES, dtypes)
+    before, n = [g.clone() for g in grads], norm64(grads)
+    versions = [g._version for g in grads]
+    norm = clip_gradients(grads, max_norm)
+    assert norm.dtype == torch.float32 and norm.dim() == 0 and norm.is_cuda and abs(float(norm) - n) <= 1e-7 * n
+    factor = min(1.0, max_norm / (n + 1e-6))
+    for g, b in zip(grads, before):
+        if factor == 1.0:
+            assert torch.equal(g, b)
+        close(g, b.double() * factor, g.dtype)
+    assert all(g._version > v for g, v in zip(grads, versions))
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                             (torch.bfloat16, torch.float32)])
+def test_into_others_at_any_alignment(device, dtype, out_dtype):
+    sizes = [1, 7, 8, 9, 8191, 8192, 8200, 30000, 2, 65537]
+    for shift_in, shift_out in ((0, 0), (1, 0), (0, 3), (5, 2)):
+        flat = seeded_normal((sum(sizes) + 8,), 3, torch.float32).to(dtype).to(device)
+        into = torch.full((sum(sizes) + 8,), 77.0, dtype=out_dtype, device=device)
+        keep = flat.clone()
+        grads = list(flat[shift_in:shift_in + sum(sizes)].split(sizes))
+        outs = list(into[shift_out:shift_out + sum(sizes)].split(sizes))
+        n = norm64(grads)
+        norm = clip_gradients(grads, 2.0, out=outs)
+        assert abs(float(norm) - n) <= 1e-7 * n and torch.equal(flat, keep)
+        for g, o in zip(grads, outs):
+            close(o, g.double() * (2.0 / (n + 1e-6)), out_dtype)
+        assert bool((into[:shift_out] == 77).all()) and bool((into[shift_out + sum(sizes):] == 77).all())
+
+
+def test_more_tensors_than_a_launch(device):
+    grads = make(device, [(i % 13 + 1, i % 7 + 1) for i in range(500)], (torch.float32, torch.bfloat16))
+    n, before = norm64(grads), [g.clone() for g in grads]
+    norm = clip_gradients(grads, 1.0)
+    assert abs(float(norm) - n) <= 1e-7 * n
+    for g, b in zip(grads, before):
+        close(g, b.double() * (1.0 / (n + 1e-6)), g.dtype)
+
+
+def test_largest_magnitude(device):
+    grads = make(device, SIZES, (torch.float32, torch.bfloat16))
+    want = max(float(g.abs().max()) for g in grads if g.numel())
+    assert float(grad_norm(grads, math.inf)) == want
+    grads[7][5, 5] = math.nan
+    assert math.isnan(float(grad_norm(grads, math.inf))) and math.isnan(float(grad_norm(grads)))
+    grads[7][5, 5] = -math.inf
+    assert float(grad_norm(grads, math.inf)) == math.inf == float(grad_norm(grads))
+
+
+def test_values_that_squares_would_lose(device):
+    """Squares of 1e30 overflow float32 and those of 1e-30 vanish in it; beside 4,000 large values 1e7 small ones count."""
+    assert abs(float(grad_norm([torch.full((1000,), 1e30, device=device)])) / (1e30 * math.sqrt(1000)) - 1) <= 1e-7
+    assert abs(float(grad_norm([torch.full((1000,), 1e-30, device=device)])) / (1e-30 * math.sqrt(1000)) - 1) <= 1e-7
+    many = [torch.full((4000,), 3.0, device=device), torch.full((10 ** 7,), 1e-2, device=device)]
+    assert abs(float(grad_norm(many)) / norm64(many) - 1) <= 1e-7
+
+
+def test_not_finite(device):
+    for bad, check in ((math.nan, torch.isnan), (math.inf, None)):
+        grads = make(device, [(10,), (20,)])
+        grads[0][3] = bad
+        before = [g.clone() for g in grads]
+        with pytest.raises(RuntimeError):
+            clip_gradients(grads, 1.0, error_if_nonfinite=True)
+        assert all(torch.equal(a, b) or torch.isnan(a).any() for a, b in zip(grads, before)) and torch.equal(grads[1], before[1])
+        norm = clip_gradients(grads, 1.0)
+        assert not math.isfinite(float(norm))
+        if check:
+            assert all(bool(check(g).all()) for g in grads)
+        else:
+            assert not grads[1].any() and math.isnan(float(grads[0][3])) and not grads[0][:3].any()
+
+
+def test_layouts(device):
+    base = seeded_normal((40, 60), 1, torch.float32).to(device)
+    grads = [base.t(), seeded_normal((10, 8), 2, torch.float32).to(device)[:, ::2], seeded_normal((9,), 3, torch.float32).to(device)]
+    n, before = norm64(grads), [g.clone() for g in grads]
+    norm = clip_gradients(grads, 1.0)
+    assert abs(float(norm) - n) <= 1e-7 * n
+    for g, b in zip(grads, before):
+        close(g, b.double() / (n + 1e-6), torch.float32)
+    outs = [torch.zeros(60, 40, device=device).t().contiguous().t(), torch.zeros(10, 4, device=device), torch.zeros(9, device=device)]
+    n = norm64(grads)
+    clip_gradients(grads, 0.25, out=outs)
+    for g, o in zip(grads, outs):
+        close(o, g.double() * (0.25 / (n + 1e-6)), torch.float32)
+
+
+def test_parameters(device):
+    """As torch.nn.utils.clip_grad_norm_ on a module, whose parameters without a gradient are passed over."""
+    model = torch.nn.Sequential(torch.nn.Linear(33, 65), torch.nn.Linear(65, 3)).to(device)
+    unused = torch.nn.Parameter(torch.zeros(5, device=device))
+    x = seeded_normal((20, 33), 1, torch.float32).to(device)
+
+    def grads():
+        model.zero_grad()
+        (model(x).square().sum() * 10).backward()
+        return [p.grad for p in model.parameters()]
+    want = [g.clone() for g in grads()]
+    n = norm64(want)
+    got = clip_grad_norm_([*model.parameters(), unused], 0.7)
+    assert abs(float(got) - n) <= 1e-7 * n and unused.grad is None
+    for p, w in zip(model.parameters(), want):
+        close(p.grad, w.double() * (0.7 / (n + 1e-6)), torch.float32)
+    theirs = grads()
+    torch.nn.utils.clip_grad_norm_(model.parameters(), 0.7)
+    for a, w in zip(theirs, want):   # one formula: float32's roundings apart
+        assert bool(((a.double() - w.double() * (0.7 / (n + 1e-6))).abs() <= 1e-5 * w.abs()).all())
+    assert float(clip_grad_norm_([unused], 1.0)) == 0.0 == float(clip_gradients([], 1.0))
+    assert abs(float(clip_grad_norm_(model[0].weight, 1e9)) - norm64([model[0].weight.grad])) <= 1e-6
+
+
+def test_shared_memory(device):
+    a, b = (seeded_normal((100,), i, torch.float32).to(device) for i in (1, 2))
+    for grads, out in (([a, a], None), ([a[:60], a[50:]], None), ([a, b], [b, a]), ([a[:50]], [a[10:60]]),
+                       ([a[:50], b[:50]], [b[50:], b[50:]]), ([a.bfloat16()], None)):
+        if grads[0].dtype == torch.bfloat16:   # a float32 output over its bfloat16 gradient
+            half = grads[0]
+            out = [torch.empty(0, device=device).set_(half.untyped_storage(), 0, (50,), (1,))]
+            grads = [half[:50]]
+        keep = a.clone()
+        with pytest.raises(ValueError, match="share"):
+            clip_gradients(grads, 1.0, out=out)
+        assert torch.equal(a, keep)
+    want = norm64([a, a])
+    assert abs(float(grad_norm([a, a])) - want) <= 1e-7 * want
+    outs = [torch.empty_like(a), torch.empty_like(a)]
+    clip_gradients([a, a], 1.0, out=outs)   # read twice, written apart
+    assert torch.equal(outs[0], outs[1])
+    other, keep = a.clone(), b.clone()
+    clip_gradients([a, b], 1.0, out=[a, torch.empty_like(b)])   # one in place, one not
+    close(a, other.double() / (norm64([other, b]) + 1e-6), torch.float32)
+    assert torch.equal(b, keep)
+
+
+def test_on_a_stream_and_replayed(device):
+    grads = make(device, SIZES, (torch.float32, torch.bfloat16))
+    outs = [torch.empty_like(g) for g in grads]
+    first = [clip_gradients(grads, 1.0, out=outs)] + [o.clone() for o in outs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = [clip_gradients(grads, 1.0, out=outs)] + [o.clone() for o in outs]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_gradients(grads, 1.0, out=outs)
+    for seed in (1, 2, 3):
+        for g, new in zip(grads, make(device, SIZES, (torch.float32, torch.bfloat16), seed)):
+            g.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        held = [norm.clone()] + [o.clone() for o in outs]
+        again = [clip_gradients(grads, 1.0, out=outs)] + outs
+        assert all(torch.equal(x, y) for x, y in zip(held, again))
+
+
+def test_refused(device):
+    g = [torch.zeros(5, device=device)]
+    for args, kwargs, error in (((g, -1.0), {}, ValueError), ((g, math.nan), {}, ValueError), ((g, 1.0, 1.0), {}, ValueError),
+                                (([torch.zeros(5, device=device, dtype=torch.float16)], 1.0), {}, TypeError),
+                                ((g, 1.0), {"out": []}, ValueError), ((g, 1.0), {"out": [torch.zeros(4, device=device)]}, ValueError),
+                                ((g, 1.0), {"out": [torch.zeros(5, device=device, dtype=torch.bfloat16)]}, TypeError)):
+        with pytest.raises(error):
+            clip_gradients(*args, **kwargs)

@@ -1,0 +1,128 @@
+"""Refusals of the query and key norms and of the gradient norm (no GPU needed)."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mind_amd import _lib
+from mind_amd.esa.gradients import _Lists, _separate, clip_gradients, grad_norm
+from mind_amd.esa.qk_norm import qk_norm_rotary, rotary_frequencies
+
+
+def test_frequencies():
+    f = rotary_frequencies(8, 10000.0)
+    assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
+    for bad in (0, 7, -2):
+        with pytest.raises(ValueError):
+            rotary_frequencies(bad)
+
+
+def _x(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+POS, FREQ = torch.arange(6), rotary_frequencies(16)
+
+
+@pytest.mark.parametrize("args,error", [
+    (dict(q=_x(6, 2, 20)), ValueError), (dict(q=_x(6, 32)), ValueError), (dict(q=_x(6, 2, 16, dtype=torch.float16)), TypeError),
+    (dict(q=_x(6, 0, 16)), ValueError), (dict(q=_x(1, 2049, 16)), ValueError),
+    (dict(k=_x(5, 2, 16)), ValueError), (dict(k=_x(6, 2, 32)), ValueError), (dict(k=_x(6, 2, 16, dtype=torch.bfloat16)), ValueError),
+    (dict(q_weight=_x(8)), ValueError), (dict(q_weight=_x(16, dtype=torch.float64)), ValueError),
+    (dict(k=None, k_weight=_x(16)), ValueError), (dict(positions=POS), ValueError), (dict(frequencies=FREQ), ValueError),
+    (dict(positions=POS.float(), frequencies=FREQ), TypeError), (dict(positions=torch.arange(12)[::2], frequencies=FREQ), TypeError),
+    (dict(positions=POS[:5], frequencies=FREQ), ValueError), (dict(positions=POS, frequencies=FREQ.float()), TypeError),
+    (dict(positions=POS, frequencies=FREQ[:3]), ValueError), (dict(positions=POS, frequencies=rotary_frequencies(24)), ValueError),
+    (dict(positions=POS, frequencies=FREQ[:0]), ValueError), (dict(eps=-1e-6), ValueError), (dict(eps=math.inf), ValueError),
+    (dict(), _lib.EsaError)])   # host tensors
+def test_qk_norm_refused(args, error):
+    with pytest.raises(error):
+        qk_norm_rotary(**{"q": _x(6, 2, 16), "k": _x(6, 3, 16), **args})
+
+
+def test_qk_norm_entry_points_refuse_before_launch():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.load()
+
+    def fwd(q=16, k=16, strides=(32, 16, 32, 16), total=5, hq=2, hk=2, hd=16, dt=0, pos=16, pb=4, f=16, r=16, eps=1e-6, out=16):
+        return lib.esa_qk_norm_fwd(q, k, (ctypes.c_longlong * 4)(*strides), total, hq, hk, hd, dt, None, None, pos, pb, f, r, 0,
+                                   eps, out, 16, None)
+    assert fwd(hd=20) == -3 and fwd(dt=4) == -5 and fwd(total=-1) == -2 and fwd(hq=0) == -2 and fwd(hk=-1) == -2
+    assert fwd(hq=3000) == -2 and fwd(eps=-1.0) == -2 and fwd(r=12) == -2 and fwd(r=24) == -2 and fwd(pb=2) == -5
+    assert fwd(q=None) == -1 and fwd(k=None) == -1 and fwd(pos=None) == -1 and fwd(f=None) == -1 and fwd(out=None) == -1
+    assert fwd(q=8) == -6 and fwd(strides=(33, 16, 32, 16)) == -6 and fwd(out=20) == -6
+    assert fwd(total=0, q=None, out=None) == 0
+    assert lib.esa_qk_norm_fwd(16, 16, None, 5, 2, 2, 16, 0, None, None, None, 0, None, 0, 0, 0.0, 16, 16, None) == -1
+    n = ctypes.c_size_t(0)
+    assert lib.esa_qk_norm_bwd_workspace_size(1000, 16, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.esa_qk_norm_bwd_workspace_size(1000, 17, ctypes.byref(n)) == -3
+    s = (ctypes.c_longlong * 4)(32, 16, 32, 16)
+
+    def bwd(gq=16, dq=16, dwq=16, ws=16, nbytes=1 << 20):
+        return lib.esa_qk_norm_bwd(gq, 16, 16, 16, s, 5, 2, 2, 16, 0, None, None, None, 0, None, 0, 0, 0.0, dq, 16, dwq, None, ws,
+                                   nbytes, None)
+    assert bwd(gq=None) == -1 and bwd(dq=None) == -1 and bwd(ws=None) == -1 and bwd(nbytes=4) == -4 and bwd(gq=4) == -6
+
+
+def test_gradient_norm_refuses_host_tensors():
+    with pytest.raises(_lib.EsaError):
+        grad_norm([torch.zeros(4)])
+    with pytest.raises(TypeError):
+        clip_gradients([torch.zeros(4, dtype=torch.float64)], 1.0)
+    assert float(grad_norm([])) == 0.0
+
+
+class _Spans(_Lists):
+    def __init__(self, spans):
+        self.n, self._spans = len(spans), np.array(spans, dtype=np.int64).reshape(-1, 2)
+
+    def spans(self):
+        return self._spans[:, 0], self._spans[:, 1]
+
+
+def test_separate_against_every_pair():
+    rng = np.random.default_rng(0)
+    for trial in range(2000):
+        n = int(rng.integers(1, 5))
+        first = rng.integers(0, 24, size=(2, n)) * 2
+        size = rng.integers(0, 5, size=(2, n)) * 2
+        if trial % 3 == 0:
+            first[1], size[1] = first[0], size[0]
+        dst, src = (_Spans([(f, f + s) for f, s in zip(first[i], size[i])]) for i in (0, 1))
+
+        def shares(a, b):
+            return max(a[0], b[0]) < min(a[1], b[1])
+        d, s = dst._spans.tolist(), src._spans.tolist()
+        apart = not any(shares(d[i], d[j]) for i in range(n) for j in range(i))
+        assert _separate(dst, dst) == apart
+        want = apart and not any(shares(d[i], s[j]) and not (i == j and d[i] == s[j]) for i in range(n) for j in range(n))
+        assert _separate(dst, src) == want
+
+
+def test_gradient_entry_points_refuse_before_launch():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib, n = _lib.load(), ctypes.c_size_t(0)
+
+    def lists(ptrs=(16,), counts=(10,), codes=(0,)):
+        k = len(ptrs)
+        return (ctypes.c_void_p * k)(*ptrs), (ctypes.c_longlong * k)(*counts), (ctypes.c_int * k)(*codes)
+
+    def norm(n_=1, out=16, ws=16, nbytes=1 << 20, **kw):
+        p, c, d = lists(**kw)
+        return lib.esa_grad_norm(n_, p, c, d, 0, out, ws, nbytes, None)
+    assert norm(n_=-1) == -2 and norm(counts=(-1,)) == -2 and norm(codes=(3,)) == -5 and norm(ptrs=(None,)) == -1
+    assert norm(ptrs=(18,)) == -6 and norm(ptrs=(17,), codes=(1,)) == -6 and norm(out=None) == -1 and norm(ws=None) == -1
+    assert norm(nbytes=4) == -4
+    p, c, d = lists()
+    assert lib.esa_grad_norm_workspace_size(1, c, ctypes.byref(n)) == 0 and n.value == 8
+    assert lib.esa_grad_norm_workspace_size(1, None, ctypes.byref(n)) == -1
+
+    def clip(out=(16,), out_codes=(0,), max_norm=1.0, norm_at=16, **kw):
+        p, c, d = lists(**kw)
+        return lib.esa_grad_clip(1, p, (ctypes.c_void_p * 1)(*out), c, d, (ctypes.c_int * 1)(*out_codes), max_norm, norm_at, None)
+    assert clip(out=(None,)) == -1 and clip(out=(18,)) == -6 and clip(out_codes=(1,)) == -5 and clip(norm_at=None) == -1
+    assert clip(max_norm=-1.0) == -2 and clip(max_norm=float("nan")) == -2
