@@ -1952,7 +1952,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   uint32_t rKey = 0;
   bool odd = false;   // edge mask: this thread staged an infinity or a NaN of a key
   const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
-  RelSums<4> sums(sRel, a.rel.stride, T::kThreads / 64, wave, grp);
+  RelSums sums(sRel, a.rel.stride, wave);
   if (BIAS) {
     rel_load_line(sRel, a.rel, head, tid, T::kThreads);
     sums.clear(a.rel.stride, lane);
@@ -1980,6 +1980,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
           const bool near = BIAS && rel_near(a.rel, base, kF32Stage, 16 * QB, far_hi);
           const float far = BIAS ? sRel[far_hi ? a.rel.stride - 1 : 0] : 0.f;
           float far_sum = 0.f;
+          f32x4 kept[QB][KB];   // a near stage's dS
           auto block = [&](int kb) {
             f32x4 x[NR], s[QB], ds[QB];
             f32_rows<HD>(x, sK[buf], 16 * kb, c16, grp);
@@ -2002,10 +2003,12 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
                 ds[b][r] = p * (dp - rs[b].y);
                 if (MASKED || tail)
                   ds[b][r] = admissible_f32<MASKED>(k0 + key, phi, own.tok[b], pn, node[b]) ? ds[b][r] : 0.f;
-                if (BIAS && near) sums.add(entry, ds[b][r]);
                 if (BIAS && !near) far_sum += ds[b][r];
               }
             }
+            if (BIAS && near)
+#pragma unroll
+              for (int b = 0; b < QB; ++b) kept[b][kb] = ds[b];
             if constexpr (decltype(checked)::value)
               f32_gather_admissible<HD>(acc, sK[buf], 16 * kb, ds, c16, grp, sN[buf], k0, phi, own.tok, node);
             else
@@ -2019,8 +2022,12 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
             for (int kb = 0; kb < KB; ++kb) block(kb);
           }
           if (BIAS) {
-            if (near) sums.stage_done(base, a.rel.stride, lane);
-            else (far_hi ? sums.hi : sums.lo) += far_sum;
+            if (near) {
+#pragma unroll
+              for (int b = 0; b < QB; ++b) sums.stage16(kept[b], base, 16 * b, lane);
+            } else {
+              (far_hi ? sums.hi : sums.lo) += far_sum;
+            }
           }
         });
   };
@@ -2815,7 +2822,7 @@ int f32_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipS
   a.rows = r.rows;
   a.dq = static_cast<float*>(c.dq); a.dk = static_cast<float*>(c.dk); a.dv = static_cast<float*>(c.dv);
   auto line = [&](int) { return r.bias.stride * sizeof(float); };
-  auto sums = [&](int waves) { return rel_dq_floats(r.bias.stride, waves, 4) * sizeof(float); };
+  auto sums = [&](int waves) { return rel_dq_floats(r.bias.stride, waves) * sizeof(float); };
   if (c.total_q > 0)
     ESA_TIMED(esa_profile::kAttnBwdDq, st,
               ESA_F32_REL_LAUNCH(attn_dq_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c), sums, st, a));

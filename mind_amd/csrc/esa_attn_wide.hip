@@ -313,19 +313,17 @@ constexpr int kWGroup = kWaves * kTile;   // 128 owned tokens per block
 
 // x[r] = c s[r] + bias - sub of a 32 x 32 tile whose keys (queries) lie in the registers: entry base + at + 16 (r / 8)
 // + r % 8 of the line, or one value for the tile.
-DEVI bool rel_scores(const RelBias& rel, const float* line, int base, int at, const f32x16& s, float c, float sub,
-                     float (&x)[16]) {
-  bool far_hi;
-  if (rel_near(rel, base, kTile, kTile, far_hi)) {
+DEVI void rel_scores(bool near, bool far_hi, const RelBias& rel, const float* line, int base, int at, const f32x16& s,
+                     float c, float sub, float (&x)[16]) {
+  if (near) {
     const float* b = line + base + at;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = fmaf(s[r], c, b[16 * (r >> 3) + (r & 7)] - sub);
-    return true;
-  }
-  const float b = line[far_hi ? rel.stride - 1 : 0] - sub;
+  } else {
+    const float b = line[far_hi ? rel.stride - 1 : 0] - sub;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) x[r] = fmaf(s[r], c, b);
-  return false;
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(s[r], c, b);
+  }
 }
 
 // ------------------------------------------------------------------ forward
@@ -405,7 +403,10 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
           }
           float p[16];
           if (BIAS) {   // scores and m_run in powers of two, c s + bias log2(e)
-            rel_scores(a.rel, sRel, rel_base(a.rel, k0, g.x + wave * kTile, shift), 8 * h - col, s, a.c, 0.f, p);
+            const int base = rel_base(a.rel, k0, g.x + wave * kTile, shift);
+            bool far_hi;
+            const bool near = rel_near(a.rel, base, kTile, kTile, far_hi);
+            rel_scores(near, far_hi, a.rel, sRel, base, 8 * h - col, s, a.c, 0.f, p);
             if (ONLINE) {
               float mt = p[0];
 #pragma unroll
@@ -482,7 +483,7 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
 // dS = P (dP - D), dQ^T += K^T dS^T.  Also writes the dK/dV pass's row
 // statistics {-LSE2 / c, -D} of its queries.
 template <int HD, bool DROP, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && !DROP ? ESA_WIDE_WAVES_DQ64 : 1)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && !DROP && !BIAS ? ESA_WIDE_WAVES_DQ64 : 1)))
 void wide_dq_kernel(const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
   __shared__ __align__(16) bf16 sK[2][NO * kWTokPad * 8];
@@ -525,7 +526,7 @@ void wide_dq_kernel(const WideArgs a) {
   const int n_stages = (n_tiles + 1) >> 1;
   const f32x16 zero = {};
   const int shift = BIAS ? a.shift[item] : 0;
-  RelSums<2> sums(sRel, a.rel.stride, kWaves, wave, h);
+  RelSums sums(sRel, a.rel.stride, wave);
   if (BIAS) {
     rel_load_line(sRel, a.rel, head, tid, 256);
     sums.clear(a.rel.stride, lane);
@@ -545,7 +546,11 @@ void wide_dq_kernel(const WideArgs a) {
       [&](int buf, int st) {
         if (!active) return;
         const int base = BIAS ? rel_base(a.rel, z0 + st * kWStage, g.x + wave * kTile, shift) : 0;
-        bool any_near = false;
+        bool far_hi = false;
+        const bool near = BIAS && rel_near(a.rel, base, kWStage, kTile, far_hi);
+        float kept[2][16];   // a near stage's dS
+#pragma unroll
+        for (int r = 0; r < 16; ++r) kept[1][r] = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           if (2 * st + u >= n_tiles) break;
@@ -562,8 +567,7 @@ void wide_dq_kernel(const WideArgs a) {
               s[r] = (unsigned)(k0 + row_local(r, h) - g.z) < (unsigned)(g.w - g.z) ? s[r] : -INFINITY;
           }
           float ds[16];
-          bool near = false;
-          if (BIAS) near = rel_scores(a.rel, sRel, base + u * kTile, 8 * h - col, s, a.c, lse2, ds);
+          if (BIAS) rel_scores(near, far_hi, a.rel, sRel, base + u * kTile, 8 * h - col, s, a.c, lse2, ds);
           if (DROP) {
             float dpk[16];
 #pragma unroll
@@ -578,14 +582,13 @@ void wide_dq_kernel(const WideArgs a) {
           }
           if (BIAS) {
             if (near) {
-              any_near = true;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) sums.add(base + u * kTile + 8 * h - col + 16 * (r >> 3) + (r & 7), ds[r]);
+              for (int r = 0; r < 16; ++r) kept[u][r] = ds[r];
             } else {
               float x = 0.f;
 #pragma unroll
               for (int r = 0; r < 16; ++r) x += ds[r];
-              (base + u * kTile > a.rel.reach + kRelPad ? sums.hi : sums.lo) += x;
+              (far_hi ? sums.hi : sums.lo) += x;
             }
           }
 #pragma unroll
@@ -593,7 +596,7 @@ void wide_dq_kernel(const WideArgs a) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[m] = mfma32(tr_dims<NO>(sK[buf], m, 2 * u + j, lane), cvt8(ds + 8 * j), acc[m]);
         }
-        if (BIAS && any_near) sums.stage_done(base, a.rel.stride, lane);
+        if (BIAS && near) sums.stage32(kept[0], kept[1], base, lane);
       });
   if (BIAS) rel_fold(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, kWaves, wave, lane, tid, 256);
   if (!valid) return;
@@ -1006,7 +1009,7 @@ int wide_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hip
   if (c.total_q > 0)
     ESA_TIMED(esa_profile::kAttnBwdDq, st,
             ESA_WIDE_REL_LAUNCH(wide_dq_kernel, c.head_dim, c.dropout, dim3(wide_grid(c.total_q, c.nseg, c.heads)),
-                                rel_dq_floats(r.bias.stride, kWaves, 2) * sizeof(float), st, a));
+                                rel_dq_floats(r.bias.stride, kWaves) * sizeof(float), st, a));
   ESA_LAUNCH_CHECK();
   a.groups = r.plan_k; a.count = r.count_k; a.shift = r.shift_k;
   if (c.total_k > 0)

@@ -9,13 +9,17 @@
 // other tile has one value, which the exponent's FMA takes for free.
 //
 // The table's gradient sums dS over the pairs of a bucket, in a fixed order
-// and without global atomics: in the dQ pass each wave adds its dS by distance
-// to a ring of 128 LDS entries per lane group (lanes of a group own different
-// queries, so the lanes of one instruction never meet in an entry, and a
-// wave's LDS operations execute in order); once a stage is done, the 64
-// distances that no later key of the wave's 32 queries can reach go to the
-// wave's line.  A block folds its lines into buckets, and a last launch sums
-// the blocks.
+// and without atomics.  In the dQ pass a wave's dS of a stage (64 keys by its
+// 32 or 16 queries) lies in its lanes as rows (keys) of columns (queries).
+// Swaps between lane halves and quarters turn it into rows of 64 lanes in
+// which lane C holds distance  row - C + constant,  so a diagonal is summed by
+// one shift of the running sum by a lane and one addition per row.  What runs
+// out at lane 0 comes from a second chain that turns round instead (their
+// difference).  The sums by distance go to the wave's line in LDS, where no
+// other wave writes; a block folds its lines into buckets, and a last launch
+// sums the blocks.  (By ds_add_f32, one per score, into a ring of distances per
+// wave, about 160 cycles an instruction, the dQ pass took 6.2 ms instead of 2.0
+// at 129,850 tokens, 32 heads of 16.)
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -69,13 +73,8 @@ namespace {
 
 extern __shared__ __align__(16) float sRel[];   // the head's bias line; the dQ pass's sums behind it
 
-constexpr int kRelRing = 128;
-
-// LDS floats of the dQ pass: the bias line, then per wave a ring for each lane group and a line of sums, then the far
-// sums of every wave.
-inline size_t rel_dq_floats(int stride, int waves, int groups) {
-  return (size_t)stride + (size_t)waves * (groups * kRelRing + stride) + 2 * waves;
-}
+// LDS floats of the dQ pass: the bias line, then for each wave a line of sums, then the far sums of every wave.
+inline size_t rel_dq_floats(int stride, int waves) { return (size_t)stride * (1 + waves) + 2 * waves; }
 
 // Entry of distance 0 at key k0 and query q0 (both first of their tiles).
 DEVI int rel_base(const RelBias& r, int k0, int q0, int shift) { return k0 - q0 - shift + r.reach + kRelPad; }
@@ -90,66 +89,95 @@ DEVI void rel_load_line(float* dst, const RelBias& r, int head, int tid, int thr
   for (int i = tid; i < r.stride; i += threads) dst[i] = r.line[(size_t)head * r.stride + i];
 }
 
+// x of the next lane (lane 63: zero, or lane 0's).
+DEVI float lane_up(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x130, 0xf, 0xf, true));
+}
+DEVI float lane_round(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x134, 0xf, 0xf, true));
+}
+// a = (a's lanes 0 .. 31, b's lanes 0 .. 31), b = (a's lanes 32 .. 63, b's lanes 32 .. 63).
+DEVI void swap_halves(float& a, float& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+// Quarters of 16 lanes: a = (a0, b0, a2, b2), b = (a1, b1, a3, b3).
+DEVI void swap_quarters(float& a, float& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+
 // One wave's sums of dS by distance.
-template <int GROUPS>
 struct RelSums {
-  float* ring;    // [GROUPS][kRelRing]
-  float* line;    // [stride]
-  float* mine;    // this lane group's ring
-  int done;       // entries below are in the line (negative: none was added)
+  float* line;    // [stride], this wave's
   float lo, hi;   // this lane's sums past -reach and reach
-  DEVI RelSums(float* lds, int stride, int waves, int wave, int group)
-      : ring(lds + stride + (size_t)wave * (GROUPS * kRelRing + stride)), line(ring + GROUPS * kRelRing),
-        mine(ring + group * kRelRing), done(-1), lo(0.f), hi(0.f) {}
-  DEVI void clear(int stride, int lane) {   // ring and line are one run
-    for (int i = lane; i < GROUPS * kRelRing + stride; i += 64) ring[i] = 0.f;
+  DEVI RelSums(float* lds, int stride, int wave) : line(lds + (size_t)stride * (1 + wave)), lo(0.f), hi(0.f) {}
+  DEVI void clear(int stride, int lane) {
+    for (int i = lane; i < stride; i += 64) line[i] = 0.f;
   }
-  DEVI void add(int entry, float x) {
-    __hip_atomic_fetch_add(&mine[entry & (kRelRing - 1)], x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-  }
-  DEVI void flush(int first, int stride, int lane) {    // entries first .. first + 63
-    const int s = (first + lane) & (kRelRing - 1);
-    float x = 0.f;
+  // Adds v[row] of lane C to entry top + row - C.
+  template <int ROWS>
+  DEVI void diagonals(const float (&v)[ROWS], int top, int lane) {
+    float a = v[ROWS - 1], z = v[ROWS - 1];
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      x += ring[g * kRelRing + s];
-      ring[g * kRelRing + s] = 0.f;
+    for (int r = ROWS - 2; r >= 0; --r) {
+      a = lane_up(a) + v[r];
+      z = lane_round(z) + v[r];
     }
-    if (first + lane < stride) line[first + lane] += x;   // past it nothing was added
+    line[top - lane] += a;
+    if (lane > 64 - ROWS) line[top - lane + 64] += z - a;
   }
-  // After a stage of 64 keys (base = rel_base of its first key) with a near tile: 32 queries' entries below
-  // base + 64 - 31 are complete.
-  DEVI void stage_done(int base, int stride, int lane) {
-    flush(base - 31, stride, lane);
-    done = base + 33;
+  // Two 32 x 32 tiles of a stage (keys 16 (r / 8) + 8 (lane / 32) + r % 8 and 32 more, queries lane % 32).
+  DEVI void stage32(float (&t0)[16], float (&t1)[16], int base, int lane) {
+    float v[32];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      swap_halves(t1[r], t0[r]);   // the second tile's keys are 32 further: its queries' lanes come first
+      v[16 * (r >> 3) + (r & 7)] = t1[r];
+      v[16 * (r >> 3) + 8 + (r & 7)] = t0[r];
+    }
+    diagonals(v, base + 32, lane);
   }
-  DEVI void finish(int stride, int lane) {
-    if (done >= 0) flush(done, stride, lane);
+  // Four 16 x 16 blocks t[i][r]: keys 16 i + 4 (lane / 16) + r, queries q + lane % 16 of the wave's.
+  DEVI void stage16(f32x4 (&t)[4], int base, int q, int lane) {
+    float v[16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float w0 = t[3][r], w1 = t[2][r], w2 = t[1][r], w3 = t[0][r];   // lane quarter i is to hold block 3 - i
+      swap_halves(w0, w2);
+      swap_halves(w1, w3);
+      swap_quarters(w0, w1);
+      swap_quarters(w2, w3);
+      v[r] = w0;
+      v[4 + r] = w1;
+      v[8 + r] = w2;
+      v[12 + r] = w3;
+    }
+    diagonals(v, base + 48 - q, lane);
   }
 };
 
-// The block's dS sums by bucket: every thread of the block, after its waves' last add.  lds: as rel_dq_floats.
-template <int GROUPS>
-DEVI void rel_fold(float* lds, RelSums<GROUPS>& own, const RelBias& r, float* part, int waves, int wave, int lane,
-                   int tid, int threads) {
-  own.finish(r.stride, lane);
+// The block's dS sums by bucket: every thread of the block, after its waves' last stage.  lds: as rel_dq_floats.
+DEVI void rel_fold(float* lds, const RelSums& own, const RelBias& r, float* part, int waves, int wave, int lane, int tid,
+                   int threads) {
   float lo = own.lo, hi = own.hi;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     lo += __shfl_xor(lo, o);
     hi += __shfl_xor(hi, o);
   }
-  const size_t per = (size_t)GROUPS * kRelRing + r.stride;
-  float* far = lds + r.stride + waves * per;
+  float* far = lds + (size_t)r.stride * (1 + waves);
   if (lane == 0) {
     far[2 * wave] = lo;
     far[2 * wave + 1] = hi;
   }
   __syncthreads();
-  float* first = lds + r.stride + GROUPS * kRelRing;
+  float* first = lds + r.stride;
   for (int i = tid; i < r.stride; i += threads) {
     float x = first[i];
-    for (int w = 1; w < waves; ++w) x += first[w * per + i];
+    for (int w = 1; w < waves; ++w) x += first[w * r.stride + i];
     first[i] = x;
   }
   __syncthreads();
