@@ -543,7 +543,7 @@ ESA_API int esa_weight_grad(long long rows, int n, const void* const* g, const v
 /* A table entry of -inf leaves its pairs out; finite ones beyond +-1e4 count */
 /* as +-1e4.  A query without a key gets output 0 and lse -inf, and so does a */
 /* token in no segment.  Tensors, dtypes, head dims, dropout and lse are      */
-/* those of esa_varlen_attn_fwd, but up to 2^29 - 1 tokens of any row size.   */
+/* those of esa_varlen_attn_fwd, but up to 2^28 - 1 tokens of any row size.   */
 /* dtable [num_buckets, heads] fp32: sums of dS in a fixed order              */
 /* (deterministic; for bf16 calls their row statistic comes from the rounded  */
 /* output, relative error about 2^-10).  Workspace size from the query.       */

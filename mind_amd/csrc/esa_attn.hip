@@ -1622,7 +1622,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
     l[b] = 0.f;
   }
   const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
-  if (BIAS) rel_load_line(sRel, a.rel, head, tid, T::kThreads);
+  if (BIAS) rel_load_line<T::kThreads>(sRel, a.rel, head, tid);
   f32x4 rK[T::kPer], rV[T::kPer];
   int2 rN = make_int2(-1, -1);
   uint32_t rKey = 0;
@@ -1954,7 +1954,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
   RelSums sums(sRel, a.rel.stride, wave);
   if (BIAS) {
-    rel_load_line(sRel, a.rel, head, tid, T::kThreads);
+    rel_load_line<T::kThreads>(sRel, a.rel, head, tid);
     sums.clear(a.rel.stride, lane);
   }
   auto walk = [&](auto checked) {
@@ -2023,8 +2023,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
           }
           if (BIAS) {
             if (near) {
-#pragma unroll
-              for (int b = 0; b < QB; ++b) sums.stage16(kept[b], base, 16 * b, lane);
+              sums.stage16(kept, base, lane);
             } else {
               (far_hi ? sums.hi : sums.lo) += far_sum;
             }
@@ -2033,8 +2032,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   };
   walk(std::false_type());
   if (BIAS)
-    rel_fold(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, T::kThreads / 64, wave, lane, tid,
-             T::kThreads);
+    rel_fold<T::kThreads>(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, wave, lane, tid);
   if (MASKED && __syncthreads_or(odd)) {   // again, over the admissible pairs alone
 #pragma unroll
     for (int b = 0; b < QB; ++b)
@@ -2081,7 +2079,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   uint32_t rKey = 0;
   bool odd = false;   // edge mask: this thread staged an infinity or a NaN of a q or dO row
   const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
-  if (BIAS) rel_load_line(sRel, a.rel, head, tid, T::kThreads);
+  if (BIAS) rel_load_line<T::kThreads>(sRel, a.rel, head, tid);
   auto walk = [&](auto checked) {
     f32_stages(
         own.plo, phi, own.live,

@@ -26,6 +26,7 @@
 #include "esa_attn_tiles.h"
 #include "esa_attn_dense.h"
 #include "esa_profile.h"
+#include "esa_rel_bias.h"
 #include "../../include/esa_hip.h"
 
 namespace {
@@ -57,6 +58,7 @@ struct DenseArgs {
   int total_q, total_k, heads, tq_pad;
   float c, scale;              // c = scale * log2(e)
   bf16* o; float* lse_out; bf16* dq; bf16* dk; bf16* dv;
+  RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
 };
 
 // ------------------------------------------------------------------ block mapping
@@ -101,11 +103,15 @@ unsigned group_blocks(int groups, int H) {
 // so a stage's load is waited for on its own and the next stage's load
 // stays in flight).  The token is clamped into the tensor: a row past the
 // segment is masked in the compute whatever it holds.
+// CUT: a token at or past `end` gives a zero row (whatever the next segment
+// holds, a zero weight times it stays zero).
+template <bool CUT = false>
 DEVI i32x4 stage_chunk(const bf16* __restrict__ a, const bf16* __restrict__ b, int token, int total, int H,
-                       int head, int hf, int lane) {
+                       int head, int hf, int lane, int end = 0) {
   const bf16* base = lane < 32 ? a : b;
   const int t = min(token, total - 1);
-  return *reinterpret_cast<const i32x4*>(base + ((size_t)t * H + head) * kHd + 8 * hf);
+  const i32x4 x = *reinterpret_cast<const i32x4*>(base + ((size_t)t * H + head) * kHd + 8 * hf);
+  return CUT && token >= end ? i32x4{} : x;
 }
 constexpr uint32_t kNoLoad = 0xFFFFFFF0u;   // buffer offset past any range: the load returns zeros
 
@@ -178,6 +184,7 @@ DEVI void stage_tiles(int buf, int st, int n_tiles, Ops ops, Tile tile, int t0) 
 constexpr int kFwdTiles = ESA_FWD_TILES;
 constexpr int kFwdGroup = kWaves * kTile * kFwdTiles;   // queries per block
 
+template <bool BIAS>
 __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense_fwd_kernel(const DenseArgs a) {
   constexpr int T = kFwdTiles;
   __shared__ __align__(16) bf16 sK[2][kSplitRows];   // K rows split by dims half
@@ -192,6 +199,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
   const int4 g = a.groups[item];
 
   if (tid < 4) sOnes[tid] = (bf16)1.f;   // visible after the walk's first barrier
+  const int shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line<256>(sRel, a.rel, head, tid);
   const int o0 = g.x + wave * kTile * T;
   int t[T];
   bool valid[T], active[T];
@@ -215,13 +224,17 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
     bnd = fmaxf(bnd, valid[u] ? a.c * sqrtf(qq) * km : 0.f);   // bound b = c |q| max|k| over the segment's keys
     split_scaled(qf, a.c, qh[u], ql[u]);
   }
+  // the reference point may move between the line's ends and 0
+  if (BIAS) bnd += 2.f * a.rel.top[head];
   const bool any_active = active[0];
   const bool fixed_ref = __builtin_amdgcn_readfirstlane((int)(wave_max(bnd) <= kStaticBound)) != 0;
 
   const int n_tiles = (g.w - g.z + kTile - 1) >> 5;
   const int n_stages = (n_tiles + 1) >> 1;
   const int tok = split_tok(wave, lane), hs = split_half(lane);
-  auto gload = [&](int st) { return stage_chunk(a.k, a.v, g.z + st * kStageTok + tok, a.total_k, H, head, hs, lane); };
+  auto gload = [&](int st) {
+    return stage_chunk<BIAS>(a.k, a.v, g.z + st * kStageTok + tok, a.total_k, H, head, hs, lane, g.w);
+  };
   auto lstore = [&](int buf, i32x4 r) { put_half<kHalfRows>(lane < 32 ? sK[buf] : sV[buf], tok, hs, r); };
 
   float m_run[T];
@@ -236,9 +249,26 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
     constexpr bool ONLINE = decltype(online_tag)::value;
     auto k_rows = [&](int buf, int j) { return half_row8<kHalfRows>(sK[buf], 32 * j + kperm(col), half); };
     auto scores = [&](const bf16x8& kr, int u) { return mfma32(kr, ql[u], mfma32(kr, qh[u], zero)); };
+    // the same with the bias of tile (u, keys k0 ..) as the accumulator's seed where it differs within the tile;
+    // elsewhere `far` is the tile's one value, left to the softmax
+    auto biased_scores = [&](const bf16x8& kr, int u, int k0, bool& near, float& far) {
+      const int base = rel_base(a.rel, k0, o0 + u * kTile, shift);
+      bool far_hi;
+      near = rel_near(a.rel, base, kTile, kTile, far_hi);
+      far = near ? 0.f : sRel[far_hi ? a.rel.stride - 1 : 0];
+      if (!near) return scores(kr, u);
+      const float* line = sRel + base + 8 * half - col;
+      f32x16 b;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) b[r] = line[16 * (r >> 3) + (r & 7)];
+      return mfma32(kr, ql[u], mfma32(kr, qh[u], b));
+    };
     // Softmax of query tile u's scores s against one key tile (keys k0..),
     // then P V into acc[u].
-    auto softmax_pv = [&](int u, f32x16 s, int k0, const bf16x8& vt0, const bf16x8& vt1) {
+    // `far`: what every score of the tile is short of (BIAS).  It moves the tile's reference point instead of
+    // the scores: no operation per score.
+    auto softmax_pv = [&](int u, f32x16 s, int k0, const bf16x8& vt0, const bf16x8& vt1, float far) {
+      if (BIAS && far == -INFINITY) return;   // wave-uniform: the tile is left out
       if (k0 + kTile > g.w) {   // the segment's last, partial key tile
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = k0 + row_local(r, half) < g.w ? s[r] : -INFINITY;
@@ -249,6 +279,7 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
 #pragma unroll
         for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
         mt = fmaxf(mt, __shfl_xor(mt, 32));
+        if (BIAS) mt += far;
         const float m_new = fmaxf(m_run[u], mt);
         if (__ballot(m_new > m_run[u])) {
           const float alpha = fast_exp2(m_run[u] - (m_new == -INFINITY ? 0.f : m_new));
@@ -256,10 +287,17 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
           for (int r = 0; r < 16; ++r) acc[u][r] *= alpha;
           m_run[u] = m_new;
         }
-        const float m_use = m_run[u] == -INFINITY ? 0.f : m_run[u];
+        float m_use = m_run[u] == -INFINITY ? 0.f : m_run[u];
+        if (BIAS) m_use -= far;
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] = fast_exp2(s[r] - m_use);
       } else {
+        if (BIAS && far != m_run[u]) {   // wave-uniform, at most a few times in a walk
+          const float alpha = fast_exp2(m_run[u] - far);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[u][r] *= alpha;
+          m_run[u] = far;
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] = fast_exp2(s[r]);
       }
@@ -278,11 +316,17 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
     // query tile's softmax and P V.
     auto tile = [&](const Ops& o, int k0) {
       f32x16 s[T];
+      float far[T];
+      bool near[T];
 #pragma unroll
-      for (int u = 0; u < T; ++u) s[u] = scores(o.kr, u);
+      for (int u = 0; u < T; ++u) {
+        far[u] = 0.f;
+        if constexpr (BIAS) s[u] = biased_scores(o.kr, u, k0, near[u], far[u]);
+        else s[u] = scores(o.kr, u);
+      }
 #pragma unroll
       for (int u = 0; u < T; ++u)
-        if (u == 0 || active[u]) softmax_pv(u, s[u], k0, o.vt0, o.vt1);   // active[u]: wave-uniform
+        if (u == 0 || active[u]) softmax_pv(u, s[u], k0, o.vt0, o.vt1, far[u]);   // active[u]: wave-uniform
     };
     stage_walk(n_stages, gload, lstore, [&](int buf, int st) {
       if (!any_active) return;
@@ -318,7 +362,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
 constexpr int kDqTiles = ESA_DQ_TILES;
 constexpr int kDqGroup = kWaves * kTile * kDqTiles;   // queries per block
 
-__global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_dq_kernel(const DenseArgs a) {
+template <bool BIAS>
+__global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DQ) void dense_dq_kernel(const DenseArgs a) {
   constexpr int T = kDqTiles;
   __shared__ __align__(16) bf16 sK[2][kSplitRows];   // K rows split by dims half
   __shared__ __align__(16) bf16 sV[2][kSplitRows];   // V rows split by dims half
@@ -355,7 +400,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
       qs[u][qb] = scaled_half(*reinterpret_cast<const bf16x8*>(a.q + row + 8 * (grp & 1)), a.c, grp >= 2);
       ob[u][qb] = *reinterpret_cast<const bf16x4*>(a.dout + row + 4 * grp);
       const float lq = a.lse[(size_t)head * a.total_q + tc];
-      cl[u][qb] = splat4(lq == -INFINITY ? -INFINITY : -lq * kLog2e);   // seed of S': -LSE2
+      // seed of S': -LSE2; with a bias the lanes past the segment's end have none (their dS is summed by distance)
+      cl[u][qb] = splat4(lq == -INFINITY || (BIAS && t >= g.y) ? -INFINITY : -lq * kLog2e);
       cd[u][qb] = splat4(-dsum);                                        // seed of dP: -D
       // the dK/dV pass's row statistics of this query (rows without keys: a finite -LSE2 so that P = 0)
       if (grp == 0 && t < g.y)
@@ -366,10 +412,35 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
   const int n_tiles = (g.w - g.z + kTile - 1) >> 5;
   const int n_stages = (n_tiles + 1) >> 1;
   const int tok = split_tok(wave, lane), hs = split_half(lane);
-  auto gload = [&](int st) { return stage_chunk(a.k, a.v, g.z + st * kStageTok + tok, a.total_k, H, head, hs, lane); };
+  auto gload = [&](int st) {
+    return stage_chunk<BIAS>(a.k, a.v, g.z + st * kStageTok + tok, a.total_k, H, head, hs, lane, g.w);
+  };
   auto lstore = [&](int buf, i32x4 r) {
     put_half<kHalfRows>(lane < 32 ? sK[buf] : sV[buf], tok, hs, r);
   };
+  static_assert(!BIAS || T == 1, "one wave's stage is summed by distance at a time");
+  const int shift = BIAS ? a.shift[item] : 0;
+  RelSums sums(sRel, a.rel.stride, wave);
+  if (BIAS) {
+    rel_load_line<256>(sRel, a.rel, head, tid);
+    sums.clear(a.rel.stride, lane);
+  }
+  // BIAS: the line's entry of the stage's first key and the wave's first query; far stages: their one value
+  int base = 0;
+  f32x4 far_seed[2];   // -LSE2 plus that value
+  f32x4 kept[2][4];    // a near stage's dS by query and key block
+  // Far stages: dS summed over the keys by a product with ones, on the matrix pipe instead of an addition per score (of
+  // the bf16 dS that the dQ product takes: 2^-9 of a term, as the rounding of the row statistic).  A stage on the
+  // other side of the window takes the sum so far to its bucket.
+  f32x4 far_acc[2] = {f32x4{}, f32x4{}};
+  bool far_side = false;
+  auto far_done = [&]() {
+    if (grp == 0) (far_side ? sums.hi : sums.lo) += far_acc[0][0] + far_acc[1][0];   // every row of a product is the sum
+    far_acc[0] = far_acc[1] = f32x4{};
+  };
+  bf16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
 
   f32x4 acc[T][2];
 #pragma unroll
@@ -387,7 +458,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
     o.kt = tr_operand<kHalfRows>(sK[buf], 32 * j, c16, grp);
     return o;
   };
-  auto tile = [&](const Ops& o, int k0) {
+  auto tile = [&](auto near_tag, const Ops& o, int k0, int j) {   // j: the stage's first or second tile
+    constexpr bool NEAR = decltype(near_tag)::value;
     const bf16x8* ka = o.ka;
     const bf16x4* va = o.va;
     const bf16x8& kt = o.kt;
@@ -398,7 +470,13 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
       for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          s[u][qb][kb] = mfma16k32(ka[kb], qs[u][qb], cl[u][qb]);
+          f32x4 seed = cl[u][qb];
+          if (BIAS) {
+            const float* line = sRel + base + 32 * j + 16 * (kb - qb) + 4 * grp - c16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) seed[e] = NEAR ? cl[u][qb][0] + line[e] : far_seed[qb][e];
+          }
+          s[u][qb][kb] = mfma16k32(ka[kb], qs[u][qb], seed);
           dp[u][qb][kb] = mfma16k16(va[kb], ob[u][qb], cd[u][qb]);
         }
     if (k0 + kTile > g.w) {   // the segment's last, partial key tile
@@ -422,14 +500,48 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) ds[kb][e] = fast_exp2(s[u][qb][kb][e]) * dp[u][qb][kb][e];
+        if (BIAS) {
+          if constexpr (NEAR) {
+            kept[qb][2 * j] = ds[0];
+            kept[qb][2 * j + 1] = ds[1];
+          } else {
+            far_acc[qb] = mfma16k32(ones, cvt4x2(ds[0], ds[1]), far_acc[qb]);
+          }
+        }
         acc[u][qb] = mfma16k32(kt, cvt4x2(ds[0], ds[1]), acc[u][qb]);
       }
     }
   };
   stage_walk(n_stages, gload, lstore, [&](int buf, int st) {
     if (!active[0]) return;
-    stage_tiles(buf, st, n_tiles, ops, tile, g.z + st * kStageTok);
+    const int k0 = g.z + st * kStageTok;
+    if constexpr (BIAS) {
+      base = rel_base(a.rel, k0, o0, shift);
+      bool far_hi;
+      if (rel_near(a.rel, base, kStageTok, kTile, far_hi)) {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) kept[qb][2] = kept[qb][3] = f32x4{};
+        tile(std::true_type(), ops(buf, 0), k0, 0);
+        if (2 * st + 1 < n_tiles) tile(std::true_type(), ops(buf, 1), k0 + kTile, 1);
+        sums.stage16(kept, base, lane);
+        return;
+      }
+      const float far = sRel[far_hi ? a.rel.stride - 1 : 0];
+      if (far == -INFINITY) return;   // wave-uniform: the stage is left out
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) far_seed[qb] = splat4(cl[0][qb][0] + far);
+      if (far_hi && !far_side) {
+        far_done();
+        far_side = true;
+      }
+    }
+    tile(std::false_type(), ops(buf, 0), k0, 0);
+    if (2 * st + 1 < n_tiles) tile(std::false_type(), ops(buf, 1), k0 + kTile, 1);
   });
+  if (BIAS) {
+    far_done();
+    rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, wave, lane, tid);
+  }
 #pragma unroll
   for (int u = 0; u < T; ++u)
 #pragma unroll
@@ -455,7 +567,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DQ) void dense_
 constexpr int kDkdvTiles = ESA_DKDV_TILES;
 constexpr int kDkdvGroup = kWaves * kTile * kDkdvTiles;   // keys per block
 
-__global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DKDV) void dense_dkdv_kernel(const DenseArgs a) {
+template <bool BIAS>
+__global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DKDV) void dense_dkdv_kernel(const DenseArgs a) {
   constexpr int T = kDkdvTiles;
   __shared__ __align__(16) bf16 sQ[2][kSplitRows];     // rows split by dims half
   __shared__ __align__(16) bf16 sDO[2][kSplitRows];
@@ -494,8 +607,13 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DKDV) void dens
   const uint32_t aux0 = lane < 8 ? (uint32_t)(g.z + 16 * wave + 2 * lane) * 8u : kNoLoad;
   auto gload = [&](int st) {
     Stage2 r;
-    r.a = stage_chunk(a.q, a.dout, g.z + st * kStageTok + tok, a.total_q, H, head, hs, lane);
+    r.a = stage_chunk<BIAS>(a.q, a.dout, g.z + st * kStageTok + tok, a.total_q, H, head, hs, lane, g.w);
     r.b = bload(rx, lane < 8 ? aux0 + (uint32_t)st * (kStageTok * 8u) : aux0);
+    if (BIAS) {   // the next segment's statistics, too, stay out
+      const int q = g.z + st * kStageTok + 16 * wave + 2 * lane;
+      if (q >= g.w) r.b.x = __float_as_int(kDeadRow), r.b.y = 0;
+      if (q + 1 >= g.w) r.b.z = __float_as_int(kDeadRow), r.b.w = 0;
+    }
     return r;
   };
   auto lstore = [&](int buf, const Stage2& r) {
@@ -507,6 +625,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DKDV) void dens
     }
   };
 
+  const int shift = BIAS ? a.shift[item] : 0;
+  if (BIAS) rel_load_line<256>(sRel, a.rel, head, tid);
   f32x4 dva[T][2], dka[T][2];
 #pragma unroll
   for (int u = 0; u < T; ++u) dva[u][0] = dva[u][1] = dka[u][0] = dka[u][1] = f32x4{};
@@ -535,14 +655,33 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_DKDV) void dens
     const bf16x8& qt = o.qt;
     f32x4 s[T][2][2], dp[T][2][2];   // [u][key block][query block]
 #pragma unroll
-    for (int u = 0; u < T; ++u)
+    for (int u = 0; u < T; ++u) {
+      const int base = BIAS ? rel_base(a.rel, o0 + u * kTile, q0, shift) : 0;
+      bool far_hi = false;
+      const bool near = BIAS && rel_near(a.rel, base, kTile, kTile, far_hi);
+      f32x4 lf[2] = {ls[0], ls[1]};
+      if (BIAS && !near) {
+        const float far = sRel[far_hi ? a.rel.stride - 1 : 0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lf[0][e] += far;
+          lf[1][e] += far;
+        }
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
-          s[u][kb][qb] = mfma16k32(qa[qb], ks[u][kb], ls[qb]);
+          f32x4 seed = lf[qb];
+          if (BIAS && near) {   // the queries lie in the registers: distances fall as e rises
+            const float* line = sRel + base + 16 * (kb - qb) + c16 - 4 * grp;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) seed[e] += line[-e];
+          }
+          s[u][kb][qb] = mfma16k32(qa[qb], ks[u][kb], seed);
           dp[u][kb][qb] = mfma16k16(da[qb], vb[u][kb], dl[qb]);
         }
+    }
     if (q0 + kTile > g.w) {   // the segment's last, partial query tile
 #pragma unroll
       for (int u = 0; u < T; ++u)
@@ -628,6 +767,13 @@ __global__ __launch_bounds__(256) void dense_prep_kernel(const DensePrep p) {
   if (b < p.nb_rows) dense_rows_block(p, b, tid);
 }
 
+// The preparation with a relative position bias, then (forward) the key norms.
+__global__ __launch_bounds__(256) void dense_rel_prep_kernel(const RelPrep p, const RelPass r, const bf16* k, int nb) {
+  const int b = blockIdx.x;
+  if (b < nb) rel_prep_block(p, r, b, threadIdx.x);
+  else knorm_block(k, p.total_k, p.heads, r.tk_tiles, r.knorm, b - nb, threadIdx.x);
+}
+
 // ------------------------------------------------------------------ host side
 
 size_t al256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -696,7 +842,7 @@ int dense_attn_fwd(const DenseAttnCall& c, void* workspace, size_t workspace_byt
   a.scale = c.scale; a.c = c.scale * kLog2e;
   a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
   ESA_TIMED(esa_profile::kAttnFwd, st,
-            hipLaunchKernelGGL(dense_fwd_kernel, dim3(group_grid(c.total_q, c.nseg, c.heads, kFwdGroup)), dim3(256), 0,
+            hipLaunchKernelGGL(dense_fwd_kernel<false>, dim3(group_grid(c.total_q, c.nseg, c.heads, kFwdGroup)), dim3(256), 0,
                                st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
@@ -731,13 +877,68 @@ int dense_attn_bwd(const DenseAttnCall& c, void* workspace, size_t workspace_byt
   // dQ first: it writes the row statistics that dK/dV stages
   a.groups = p.plan_q; a.count = p.count_q;
   ESA_TIMED(esa_profile::kAttnBwdDq, st,
-            hipLaunchKernelGGL(dense_dq_kernel, dim3(group_grid(c.total_q, c.nseg, c.heads, kDqGroup)), dim3(256), 0,
+            hipLaunchKernelGGL(dense_dq_kernel<false>, dim3(group_grid(c.total_q, c.nseg, c.heads, kDqGroup)), dim3(256), 0,
                                st, a));
   ESA_LAUNCH_CHECK();
   a.groups = p.plan_k; a.count = p.count_k;
   ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
-            hipLaunchKernelGGL(dense_dkdv_kernel, dim3(group_grid(c.total_k, c.nseg, c.heads, kDkdvGroup)), dim3(256),
+            hipLaunchKernelGGL(dense_dkdv_kernel<false>, dim3(group_grid(c.total_k, c.nseg, c.heads, kDkdvGroup)), dim3(256),
                                0, st, a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+// ---- with a relative position bias (the calls of esa_rel_attn.hip)
+static DenseArgs dense_rel_args(const DenseAttnCall& c, const RelPass& r) {
+  DenseArgs a{};
+  a.q = static_cast<const bf16*>(c.q); a.k = static_cast<const bf16*>(c.k); a.v = static_cast<const bf16*>(c.v);
+  a.groups = r.plan_q; a.count = r.count_q; a.shift = r.shift_q;
+  a.total_q = c.total_q; a.total_k = c.total_k; a.heads = c.heads; a.tq_pad = r.tq_pad;
+  a.scale = c.scale; a.c = c.scale * kLog2e;
+  a.rel = r.bias;
+  return a;
+}
+
+int dense_rel_fwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st) {
+  if (c.head_dim != kHd || c.dropout) return wide_rel_fwd(c, r, p, st);
+  p.gtok_q = kFwdGroup;
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            hipLaunchKernelGGL(dense_rel_prep_kernel, dim3(nb + r.tk_tiles), dim3(256), 0, st, p, r,
+                               static_cast<const bf16*>(c.k), nb));
+  ESA_LAUNCH_CHECK();
+  if (c.total_q == 0) return ESA_OK;
+  DenseArgs a = dense_rel_args(c, r);
+  a.knorm = r.knorm; a.tk_tiles = r.tk_tiles;
+  a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
+  ESA_TIMED(esa_profile::kAttnFwd, st,
+            hipLaunchKernelGGL(dense_fwd_kernel<true>, dim3(group_grid(c.total_q, c.nseg, c.heads, kFwdGroup)), dim3(256),
+                               r.bias.stride * sizeof(float), st, a));
+  ESA_LAUNCH_CHECK();
+  return ESA_OK;
+}
+
+int dense_rel_bwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st) {
+  if (c.head_dim != kHd || c.dropout) return wide_rel_bwd(c, r, p, st);
+  static_assert(kDqGroup == kGroupTok && kDkdvGroup == kGroupTok, "the table's partial sums are sized by groups of 128");
+  const int nb = rel_prep_blocks(p);
+  ESA_TIMED(esa_profile::kAttnPrep, st,
+            hipLaunchKernelGGL(dense_rel_prep_kernel, dim3(nb), dim3(256), 0, st, p, r, nullptr, nb));
+  ESA_LAUNCH_CHECK();
+  DenseArgs a = dense_rel_args(c, r);
+  a.out = static_cast<const bf16*>(c.out_in); a.dout = static_cast<const bf16*>(c.dout);
+  a.lse = c.lse_in; a.aux = r.rows; a.aux_out = r.rows;
+  a.dq = static_cast<bf16*>(c.dq); a.dk = static_cast<bf16*>(c.dk); a.dv = static_cast<bf16*>(c.dv);
+  if (c.total_q > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDq, st,
+              hipLaunchKernelGGL(dense_dq_kernel<true>, dim3(group_grid(c.total_q, c.nseg, c.heads, kDqGroup)), dim3(256),
+                                 rel_dq_floats(r.bias.stride, kWaves) * sizeof(float), st, a));
+  ESA_LAUNCH_CHECK();
+  a.groups = r.plan_k; a.count = r.count_k; a.shift = r.shift_k;
+  if (c.total_k > 0)
+    ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
+              hipLaunchKernelGGL(dense_dkdv_kernel<true>, dim3(group_grid(c.total_k, c.nseg, c.heads, kDkdvGroup)),
+                                 dim3(256), r.bias.stride * sizeof(float), st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }

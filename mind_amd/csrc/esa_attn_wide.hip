@@ -328,7 +328,7 @@ DEVI void rel_scores(bool near, bool far_hi, const RelBias& rel, const float* li
 
 // ------------------------------------------------------------------ forward
 template <int HD, bool DROP, bool BIAS>
-__global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && BIAS && !DROP ? 3 : 1))) void wide_fwd_kernel(const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
   __shared__ __align__(16) bf16 sK[2][NO * kWTokPad * 8];
   __shared__ __align__(16) bf16 sV[2][NO * kWTokPad * 8];
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void wide_fwd_kernel(const WideArgs a) {
   const int n_stages = (n_tiles + 1) >> 1;
   const f32x16 zero = {};
   const int shift = BIAS ? a.shift[item] : 0;
-  if (BIAS) rel_load_line(sRel, a.rel, head, tid, 256);
+  if (BIAS) rel_load_line<256>(sRel, a.rel, head, tid);
   auto run = [&](auto online_tag) {
   constexpr bool ONLINE = decltype(online_tag)::value;
   wide_walk(
@@ -528,7 +528,7 @@ void wide_dq_kernel(const WideArgs a) {
   const int shift = BIAS ? a.shift[item] : 0;
   RelSums sums(sRel, a.rel.stride, wave);
   if (BIAS) {
-    rel_load_line(sRel, a.rel, head, tid, 256);
+    rel_load_line<256>(sRel, a.rel, head, tid);
     sums.clear(a.rel.stride, lane);
   }
   wide_walk(
@@ -598,7 +598,7 @@ void wide_dq_kernel(const WideArgs a) {
         }
         if (BIAS && near) sums.stage32(kept[0], kept[1], base, lane);
       });
-  if (BIAS) rel_fold(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, kWaves, wave, lane, tid, 256);
+  if (BIAS) rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)item * H + head) * a.rel.buckets, wave, lane, tid);
   if (!valid) return;
   store_acc<HD>(a.dq + ((size_t)t * H + head) * HD, acc, a.scale, h);
 }
@@ -644,7 +644,7 @@ void wide_dkdv_kernel(const WideArgs a) {
   const int n_stages = (n_tiles + 1) >> 1;
   struct Stage { WStage<HD> rows; float2 st; uint32_t key; };
   const int shift = BIAS ? a.shift[item] : 0;
-  if (BIAS) rel_load_line(sRel, a.rel, head, tid, 256);
+  if (BIAS) rel_load_line<256>(sRel, a.rel, head, tid);
   wide_walk(
       n_stages,
       [&](int st) {

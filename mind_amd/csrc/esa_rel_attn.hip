@@ -1,7 +1,8 @@
 // Entry points of the varlen attention with a learned bias by relative
 // position: argument checks, the workspace, the last sum of the table's
-// gradient.  The passes are the unmasked kernels' own (esa_attn_wide.hip for
-// bf16, esa_attn.hip for fp32); esa_rel_bias.h has the bias.
+// gradient.  The passes are the unmasked kernels' own (esa_attn_dense.hip and
+// esa_attn_wide.hip for bf16, esa_attn.hip for fp32); esa_rel_bias.h has the
+// bias.
 #include <algorithm>
 
 #include "esa_rel_bias.h"
@@ -72,7 +73,7 @@ int check(int batch, int total_q, int total_k, int heads, int head_dim, int dtyp
   if (head_dim != 16 && head_dim != 24 && head_dim != 32 && head_dim != 64) return ESA_ERR_HEAD_DIM;
   if (dtype != ESA_BF16 && dtype != ESA_F32) return ESA_ERR_DTYPE;
   // token offsets and distances (a query offset of up to 2^30 among them) stay within 32 bits
-  if (batch < 1 || heads < 1 || total_q < 0 || total_k < 0 || total_q >= 1 << 29 || total_k >= 1 << 29) return ESA_ERR_SHAPE;
+  if (batch < 1 || heads < 1 || total_q < 0 || total_k < 0 || total_q >= 1 << 28 || total_k >= 1 << 28) return ESA_ERR_SHAPE;
   if ((groups_most(std::max(total_q, total_k), batch) + 1) * (size_t)heads >= (size_t)1 << 31) return ESA_ERR_SHAPE;
   if (!starts) return ESA_ERR_NULL;
   if (buckets < 1 || buckets > kRelMaxBuckets || side < 1 || side > kRelMaxBuckets / 2 ||
@@ -125,6 +126,7 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
   p.zero_k = static_cast<uint4*>(c.dk); p.zero_v = static_cast<uint4*>(c.dv);
   p.lse = backward ? nullptr : c.lse;
   p.backward = backward;
+  p.gtok_q = kGroupTok;
   p.key_pairs = backward && c.dropout && dtype == ESA_BF16;   // the bf16 dK/dV pass shares its hashes by key pairs
 }
 
@@ -168,7 +170,7 @@ int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* ta
   fill(w, static_cast<char*>(workspace), table, table_dtype, num_buckets, bucket_starts, num_starts, q_start, c, dtype, false, r,
        p);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return dtype == ESA_BF16 ? wide_rel_fwd(c, r, p, st) : f32_rel_fwd(c, r, p, st);
+  return dtype == ESA_BF16 ? dense_rel_fwd(c, r, p, st) : f32_rel_fwd(c, r, p, st);
 }
 
 int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -199,7 +201,7 @@ int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void*
   RelPrep p{};
   fill(w, static_cast<char*>(workspace), table, table_dtype, num_buckets, bucket_starts, num_starts, q_start, c, dtype, true, r, p);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  rc = dtype == ESA_BF16 ? wide_rel_bwd(c, r, p, st) : f32_rel_bwd(c, r, p, st);
+  rc = dtype == ESA_BF16 ? dense_rel_bwd(c, r, p, st) : f32_rel_bwd(c, r, p, st);
   if (rc) return rc;
   ESA_TIMED(esa_profile::kColumnSum, st,
             hipLaunchKernelGGL(rel_reduce_kernel, dim3((unsigned)((heads * num_buckets + kReduceCols - 1) / kReduceCols)),

@@ -59,11 +59,15 @@ struct RelPrep {
   float* line; float* top; int2* ranges;
   uint4* zero_q; uint4* zero_k; uint4* zero_v; float* lse;          // out or dq; dk, dv; forward: lse
   bool backward, key_pairs;
+  int gtok_q;                                                       // tokens of a query group
 };
 constexpr int kRelClearBlocks = 16;
 inline int rel_prep_blocks(const RelPrep& p) { return 1 + (p.backward ? 1 : 0) + p.heads + kRelClearBlocks; }
 
-// esa_attn_wide.hip (bf16) and esa_attn.hip (fp32).
+// esa_attn_dense.hip (bf16: its own kernels at head dim 16 without dropout, else the next file's), esa_attn_wide.hip,
+// esa_attn.hip (fp32).
+int dense_rel_fwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st);
+int dense_rel_bwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st);
 int wide_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st);
 int wide_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st);
 int f32_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st);
@@ -85,8 +89,20 @@ DEVI bool rel_near(const RelBias& r, int base, int nk, int nq, bool& far_hi) {
   return !far_hi && base + nk - 1 > kRelPad;
 }
 
-DEVI void rel_load_line(float* dst, const RelBias& r, int head, int tid, int threads) {
-  for (int i = tid; i < r.stride; i += threads) dst[i] = r.line[(size_t)head * r.stride + i];
+constexpr int kRelMaxStride = 2 * (kRelMaxReach + kRelPad) + 1;
+// All of a thread's loads first: one wait for them in a block's start, not one an entry.
+template <int THREADS>
+DEVI void rel_load_line(float* dst, const RelBias& r, int head, int tid) {
+  constexpr int N = (kRelMaxStride + THREADS - 1) / THREADS;
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = tid + j * THREADS;
+    x[j] = i < r.stride ? r.line[(size_t)head * r.stride + i] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (tid + j * THREADS < r.stride) dst[tid + j * THREADS] = x[j];
 }
 
 // x of the next lane (lane 63: zero, or lane 0's).
@@ -117,32 +133,35 @@ struct RelSums {
   DEVI void clear(int stride, int lane) {
     for (int i = lane; i < stride; i += 64) line[i] = 0.f;
   }
-  // Adds v[row] of lane C to entry top + row - C.
-  template <int ROWS>
-  DEVI void diagonals(const float (&v)[ROWS], int top, int lane) {
-    float a = v[ROWS - 1], z = v[ROWS - 1];
+  // Adds v[row] of lane C to entry top + row - C, for two blocks of 16 rows: four chains side by side, as a shifted
+  // operand must be two instructions old.
+  DEVI void diagonals(const float (&v0)[16], int top0, const float (&v1)[16], int top1, int lane) {
+    float a0 = v0[15], z0 = v0[15], a1 = v1[15], z1 = v1[15];
 #pragma unroll
-    for (int r = ROWS - 2; r >= 0; --r) {
-      a = lane_up(a) + v[r];
-      z = lane_round(z) + v[r];
+    for (int r = 14; r >= 0; --r) {
+      a0 = lane_up(a0) + v0[r];
+      a1 = lane_up(a1) + v1[r];
+      z0 = lane_round(z0) + v0[r];
+      z1 = lane_round(z1) + v1[r];
     }
-    line[top - lane] += a;
-    if (lane > 64 - ROWS) line[top - lane + 64] += z - a;
+    line[top0 - lane] += a0;
+    if (lane > 48) line[top0 - lane + 64] += z0 - a0;
+    line[top1 - lane] += a1;
+    if (lane > 48) line[top1 - lane + 64] += z1 - a1;
   }
   // Two 32 x 32 tiles of a stage (keys 16 (r / 8) + 8 (lane / 32) + r % 8 and 32 more, queries lane % 32).
   DEVI void stage32(float (&t0)[16], float (&t1)[16], int base, int lane) {
-    float v[32];
+    float v[2][16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       swap_halves(t1[r], t0[r]);   // the second tile's keys are 32 further: its queries' lanes come first
-      v[16 * (r >> 3) + (r & 7)] = t1[r];
-      v[16 * (r >> 3) + 8 + (r & 7)] = t0[r];
+      v[r >> 3][r & 7] = t1[r];
+      v[r >> 3][8 + (r & 7)] = t0[r];
     }
-    diagonals(v, base + 32, lane);
+    diagonals(v[0], base + 32, v[1], base + 48, lane);
   }
-  // Four 16 x 16 blocks t[i][r]: keys 16 i + 4 (lane / 16) + r, queries q + lane % 16 of the wave's.
-  DEVI void stage16(f32x4 (&t)[4], int base, int q, int lane) {
-    float v[16];
+  // Four 16 x 16 blocks t[i][r]: keys 16 i + 4 (lane / 16) + r, queries lane % 16.
+  static DEVI void rows16(const f32x4 (&t)[4], float (&v)[16]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float w0 = t[3][r], w1 = t[2][r], w2 = t[1][r], w3 = t[0][r];   // lane quarter i is to hold block 3 - i
@@ -155,13 +174,25 @@ struct RelSums {
       v[8 + r] = w2;
       v[12 + r] = w3;
     }
-    diagonals(v, base + 48 - q, lane);
+  }
+  // The wave's B query blocks of 16 (B 1 or 2) by the stage's four key blocks.
+  template <int B>
+  DEVI void stage16(const f32x4 (&t)[B][4], int base, int lane) {
+    float v[2][16];
+    rows16(t[0], v[0]);
+    if constexpr (B == 2) rows16(t[1], v[1]);
+    else
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[1][r] = 0.f;
+    diagonals(v[0], base + 48, v[1], base + 32, lane);
   }
 };
 
 // The block's dS sums by bucket: every thread of the block, after its waves' last stage.  lds: as rel_dq_floats.
-DEVI void rel_fold(float* lds, const RelSums& own, const RelBias& r, float* part, int waves, int wave, int lane, int tid,
-                   int threads) {
+// Eight lanes a bucket: the outer ones hold a hundred distances and more.
+template <int THREADS>
+DEVI void rel_fold(float* lds, const RelSums& own, const RelBias& r, float* part, int wave, int lane, int tid) {
+  constexpr int waves = THREADS / 64;
   float lo = own.lo, hi = own.hi;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -175,20 +206,23 @@ DEVI void rel_fold(float* lds, const RelSums& own, const RelBias& r, float* part
   }
   __syncthreads();
   float* first = lds + r.stride;
-  for (int i = tid; i < r.stride; i += threads) {
+  for (int i = tid; i < r.stride; i += THREADS) {
     float x = first[i];
+#pragma unroll
     for (int w = 1; w < waves; ++w) x += first[w * r.stride + i];
     first[i] = x;
   }
   __syncthreads();
-  for (int b = tid; b < r.buckets; b += threads) {
+  for (int b = tid >> 3; b < r.buckets; b += THREADS / 8) {
     const int2 range = r.ranges[b];
     float x = 0.f;
-    for (int i = range.x; i < range.y; ++i) x += first[i];
-    if (b == r.far_lo)
-      for (int w = 0; w < waves; ++w) x += far[2 * w];
-    if (b == r.far_hi)
-      for (int w = 0; w < waves; ++w) x += far[2 * w + 1];
+#pragma unroll 4
+    for (int i = range.x + (tid & 7); i < range.y; i += 8) x += first[i];
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) x += __shfl_xor(x, o);
+    if (tid & 7) continue;
+#pragma unroll
+    for (int w = 0; w < waves; ++w) x += (b == r.far_lo ? far[2 * w] : 0.f) + (b == r.far_hi ? far[2 * w + 1] : 0.f);
     part[b] = x;
   }
 }
@@ -211,7 +245,7 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
     return p.cu_k[s] - p.cu_q[s] + start;
   };
   if (b == 0) {
-    seg_plan_block(p.cu_q, p.cu_k, p.nseg, kGroupTok, r.plan_q, r.count_q, tid, false, r.shift_q, shift_of);
+    seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, r.shift_q, shift_of);
     return;
   }
   b -= 1;

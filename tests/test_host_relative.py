@@ -70,7 +70,7 @@ def test_entry_points_refuse_before_launch():
                                                ctypes.byref(n))
     assert size() == 0 and n.value > 0
     assert size(hd=48) == -3 and size(dt=5) == -5 and size(batch=0) == -2 and size(h=0) == -2 and size(tq=-1) == -2
-    assert size(tk=1 << 29) == -2 and size(nb=5) == -2 and size(nb=0) == -2 and size(starts=(1, 3)) == -2
+    assert size(tk=1 << 28) == -2 and size(nb=5) == -2 and size(nb=0) == -2 and size(starts=(1, 3)) == -2
     assert size(starts=(0, 769)) == -2 and size(starts=(0, 4, 3), nb=3) == -2 and size(ns=0) == -2
     assert size(nb=300, starts=range(150)) == -2
     assert lib.esa_rel_attn_workspace_size(2, 100, 90, 4, 16, bf16, 4, None, 2, 1, ctypes.byref(n)) == -1
