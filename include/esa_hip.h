@@ -609,17 +609,19 @@ ESA_API int esa_qk_norm_bwd(const void* gq, const void* gk, const void* q, const
 /* (ESA_F32 or ESA_BF16), each contiguous, at any element alignment.          */
 /* esa_grad_norm: *norm (device fp32) = sqrt(sum of squares) (infinity 0) or  */
 /* the largest absolute value (infinity 1, a NaN staying one); squares are    */
-/* summed in fp64 in a fixed order.  esa_grad_clip: out_i = in_i *            */
-/* min(1, max_norm / (*norm + 1e-6)) (a NaN norm gives NaN), rounded once;    */
-/* out_i may be in_i; out dtypes in_i's or ESA_F32.  No tensors: norm 0.      */
+/* summed in fp64 in a fixed order.  esa_grad_clip: the same norm, and out_i  */
+/* = in_i * min(1, max_norm / (*norm + 1e-6)) (a NaN norm gives NaN), rounded */
+/* once; out_i may be in_i, but share no other memory with any tensor of the  */
+/* call; out dtypes in_i's or ESA_F32.  No tensors: norm 0.  Workspace size   */
+/* from the query (clip 1 for esa_grad_clip), 8-byte aligned.                 */
 /* ------------------------------------------------------------------------ */
-ESA_API int esa_grad_norm_workspace_size(int n, const long long* counts, size_t* bytes);
+ESA_API int esa_grad_workspace_size(int n, const long long* counts, int clip, size_t* bytes);
 ESA_API int esa_grad_norm(int n, const void* const* in, const long long* counts, const int* dtypes,
                    int infinity, float* norm, void* workspace, size_t workspace_bytes,
                    void* stream);
 ESA_API int esa_grad_clip(int n, const void* const* in, void* const* out, const long long* counts,
-                   const int* in_dtypes, const int* out_dtypes, float max_norm,
-                   const float* norm, void* stream);
+                   const int* in_dtypes, const int* out_dtypes, int infinity, float max_norm,
+                   float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Profiling hook (no counterpart in the reference; used by the benchmark).  */

@@ -10,6 +10,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -18,6 +21,7 @@ import torch
 
 # MIND_AMD_LIB selects another build of the library (same C ABI).
 LIB_PATH = Path(os.environ.get("MIND_AMD_LIB") or Path(__file__).resolve().parent / "lib" / "libesa_hip.so")
+TENSORS_PATH = Path(__file__).resolve().parent / "lib" / "esa_tensors.so"
 
 ESA_F32 = 0
 ESA_BF16 = 1
@@ -136,13 +140,11 @@ _PROTOS = {
     "esa_qk_norm_bwd": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_longlong), _c_int, _c_int, _c_int, _c_int,
                                  _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_f, _vp, _vp, _vp, _vp, _vp, _c_sz,
                                  _vp]),
-    "esa_grad_norm_workspace_size": (_c_int, [_c_int, ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(_c_sz)]),
+    "esa_grad_workspace_size": (_c_int, [_c_int, _vp, _c_int, ctypes.POINTER(_c_sz)]),   # arrays as bytes
     # n in[] counts[] dtypes[] infinity | norm ws bytes stream
-    "esa_grad_norm": (_c_int, [_c_int, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_longlong), ctypes.POINTER(_c_int),
-                               _c_int, _vp, _vp, _c_sz, _vp]),
-    # n in[] out[] counts[] in_dtypes[] out_dtypes[] | max_norm norm stream
-    "esa_grad_clip": (_c_int, [_c_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_longlong),
-                               ctypes.POINTER(_c_int), ctypes.POINTER(_c_int), _c_f, _vp, _vp]),
+    "esa_grad_norm": (_c_int, [_c_int, _vp, _vp, _vp, _c_int, _vp, _vp, _c_sz, _vp]),
+    # n in[] out[] counts[] in_dtypes[] out_dtypes[] | infinity max_norm norm ws bytes stream
+    "esa_grad_clip": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp, _c_int, _c_f, _vp, _vp, _c_sz, _vp]),
     "esa_mab_residual_fwd": (_c_int, [_vp, _vp, _vp, _c_i64, _c_int, _vp, _vp]),
     "esa_mab_residual_bwd": (_c_int, [_vp, _vp, _c_i64, _c_int, _vp, _vp, _vp]),
     "esa_profile_enable": (_c_int, [_c_int]),
@@ -176,6 +178,17 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+@functools.lru_cache(maxsize=1)
+def tensors():
+    """The host module that reads lists of tensors (csrc/esa_tensors.cpp), loaded once."""
+    if not TENSORS_PATH.exists():
+        raise EsaError(f"{TENSORS_PATH} is not built; run `python -m mind_amd._build`")
+    loader = importlib.machinery.ExtensionFileLoader("esa_tensors", str(TENSORS_PATH))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("esa_tensors", loader))
+    loader.exec_module(module)
+    return module
 
 
 def exported_symbols() -> list[str]:

@@ -900,7 +900,7 @@ static DenseArgs dense_rel_args(const DenseAttnCall& c, const RelPass& r) {
 }
 
 int dense_rel_fwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st) {
-  if (c.head_dim != kHd || c.dropout) return wide_rel_fwd(c, r, p, st);
+  if (c.head_dim != kHd || c.dropout || r.split.keys) return wide_rel_fwd(c, r, p, st);
   p.gtok_q = kFwdGroup;
   const int nb = rel_prep_blocks(p);
   ESA_TIMED(esa_profile::kAttnPrep, st,

@@ -81,6 +81,7 @@ struct WideArgs {
   float c, scale;
   bf16* o; float* lse_out; bf16* dq; bf16* dk; bf16* dv;
   RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
+  RelSplit split;                  // SPLIT: where the waves' parts go
 };
 
 // LDS position of staged token t in octet o of an NO-octet layout.  The
@@ -327,8 +328,9 @@ DEVI void rel_scores(bool near, bool far_hi, const RelBias& rel, const float* li
 }
 
 // ------------------------------------------------------------------ forward
-template <int HD, bool DROP, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && BIAS && !DROP ? 3 : 1))) void wide_fwd_kernel(const WideArgs a) {
+template <int HD, bool DROP, bool BIAS, bool SPLIT = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 && BIAS && !DROP ? 3 : 1))) void wide_fwd_kernel(
+    const WideArgs a) {
   constexpr int HP = (HD + 31) / 32 * 32, NC = (HD + 15) / 16, NM = HP / 32, NO = HP / 8;
   __shared__ __align__(16) bf16 sK[2][NO * kWTokPad * 8];
   __shared__ __align__(16) bf16 sV[2][NO * kWTokPad * 8];
@@ -340,18 +342,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
   wide_item_head<HD>(H, item, head);
   if (item >= *a.count) return;
   const int4 g = a.groups[item];
-  const int t = g.x + wave * kTile + col;
-  const bool valid = t < g.y, active = g.x + wave * kTile < g.y;
+  const int q0 = g.x + (SPLIT ? 0 : wave * kTile);   // SPLIT: the waves share their queries and divide the keys
+  const int t = q0 + col;
+  const bool valid = t < g.y, active = q0 < g.y;
   const bf16* qrow = a.q + ((size_t)(valid ? t : g.x) * H + head) * HD;
   bf16x8 qop[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) qop[c] = row_op<HD>(qrow, 2 * c + h);
   wide_zero_pad<HD>(sK[0], sK[1], sV[0], sV[1], tid);
   const uint32_t rk = DROP ? drop_row(a.drop, valid ? t : g.x, head) : 0u;
-  // the wave's bound c |q| max|k| over its partner range
+  // the wave's bound c |q| max|k| over its partner range (SPLIT: none; a walk too short to pay for the key norms)
   float km = 0.f;
-  for (int tt = (g.z >> 5) + lane; tt < ((g.w + kTile - 1) >> 5); tt += 64)
-    km = fmaxf(km, a.knorm[(size_t)head * a.tk_tiles + tt]);
+  if (!SPLIT)
+    for (int tt = (g.z >> 5) + lane; tt < ((g.w + kTile - 1) >> 5); tt += 64)
+      km = fmaxf(km, a.knorm[(size_t)head * a.tk_tiles + tt]);
   km = wave_max(km);
   float qq = 0.f;
 #pragma unroll
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
   qq += __shfl_xor(qq, 32);
   float bnd = valid ? a.c * sqrtf(qq) * km : 0.f;
   if (BIAS) bnd += a.rel.top[head];
-  const bool fixed_ref = __builtin_amdgcn_readfirstlane((int)(wave_max(bnd) <= kStaticBound)) != 0;
+  const bool fixed_ref = !SPLIT && __builtin_amdgcn_readfirstlane((int)(wave_max(bnd) <= kStaticBound)) != 0;
   f32x16 acc[NM];
 #pragma unroll
   for (int m = 0; m < NM; ++m) acc[m] = f32x16{};
@@ -392,6 +396,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           if (2 * st + u >= n_tiles) break;
+          if (SPLIT && ((2 * st + u) & 3) != wave) continue;
           const int k0 = z0 + st * kWStage + u * kTile;
           f32x16 s = zero;
 #pragma unroll
@@ -403,7 +408,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
           }
           float p[16];
           if (BIAS) {   // scores and m_run in powers of two, c s + bias log2(e)
-            const int base = rel_base(a.rel, k0, g.x + wave * kTile, shift);
+            const int base = rel_base(a.rel, k0, q0, shift);
             bool far_hi;
             const bool near = rel_near(a.rel, base, kTile, kTile, far_hi);
             rel_scores(near, far_hi, a.rel, sRel, base, 8 * h - col, s, a.c, 0.f, p);
@@ -472,10 +477,72 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
     run(std::integral_constant<bool, true>{});
   if (!valid) return;
   const float l = l_run + __shfl_xor(l_run, 32);
+  if (SPLIT) {
+    const size_t row = (((size_t)item * kWaves + wave) * H + head) * kSplitRows + col;
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (32 * m + 8 * x < HD)
+          *reinterpret_cast<float4*>(a.split.acc + row * HD + 32 * m + 8 * x + 4 * h) =
+              make_float4(acc[m][4 * x], acc[m][4 * x + 1], acc[m][4 * x + 2], acc[m][4 * x + 3]);
+    if (h == 0) a.split.ml[row] = make_float2(m_run, l);
+    return;
+  }
   store_acc<HD>(a.o + ((size_t)t * H + head) * HD, acc, l > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / l : 0.f, h);
   if (h == 0)
     a.lse_out[(size_t)head * a.total_q + t] =
         l > 0.f ? ((BIAS ? m_run : a.c * m_run) + fast_log2(l)) * kLn2 : -INFINITY;
+}
+
+// The parts of a split forward joined: a wave per (query, head).  Its lanes take the parts' maxima and sums, then the
+// dims (two rows of 32 dims at a time below head dim 64) of one part after another.
+template <int HD, bool DROP>
+__global__ __launch_bounds__(256) void wide_join_kernel(const WideArgs a) {
+  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  const int t = w / a.heads, head = w - t * a.heads;
+  if (t >= a.total_q) return;   // wave-uniform, as the next
+  const int4 where = a.split.where[t];
+  const int parts = where.y * kWaves, row = where.z;
+  if (parts == 0) return;
+  const size_t first = (size_t)where.x * kWaves;
+  auto at = [&](int i) { return ((first + i) * a.heads + head) * kSplitRows + row; };
+  float top = -INFINITY, sum = 0.f;
+  for (int i = lane; i < parts; i += 64) {
+    const float2 x = a.split.ml[at(i)];
+    const float m = x.y > 0.f ? x.x : -INFINITY, up = fmaxf(top, m);
+    if (x.y != x.y) sum = x.y;   // a NaN stays one
+    else if (m != -INFINITY) {
+      sum = sum * fast_exp2(top - up) + x.y * fast_exp2(m - up);
+      top = up;
+    }
+  }
+  const float all = wave_max(top);
+  sum = top == -INFINITY ? sum : sum * fast_exp2(top - all);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  constexpr int SIDE = HD == 64 ? 1 : 2;   // parts side by side
+  const int d = lane % (64 / SIDE), side = lane / (64 / SIDE);
+  float out = 0.f;
+  constexpr int AHEAD = 16;   // loads in flight, the last round's beyond the parts of the last part again
+  for (int i0 = side; i0 < parts; i0 += SIDE * AHEAD) {
+    float2 x[AHEAD];
+    float v[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = min(i0 + SIDE * j, parts - 1);
+      x[j] = a.split.ml[at(i)];
+      v[j] = a.split.acc[at(i) * HD + (d < HD ? d : 0)];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (i0 + SIDE * j < parts) out = x[j].y > 0.f ? fmaf(v[j], fast_exp2(x[j].x - all), out) : x[j].y != x[j].y ? x[j].y : out;
+  }
+  if (SIDE == 2) out += __shfl_xor(out, 32);
+  const float mul = sum > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / sum : sum != sum ? sum : 0.f;
+  if (side == 0 && d < HD) a.o[((size_t)t * a.heads + head) * HD + d] = (bf16)(out * mul);
+  if (lane == 0)
+    a.lse_out[(size_t)head * a.total_q + t] = sum > 0.f ? (all + fast_log2(sum)) * kLn2 : sum != sum ? sum : -INFINITY;
 }
 
 // ------------------------------------------------------------------ dQ pass
@@ -977,6 +1044,19 @@ static WideArgs wide_rel_args(const DenseAttnCall& c, const RelPass& r) {
   return a;
 }
 
+template <bool D, int HD>
+static void wide_split_hd(const DenseAttnCall& c, dim3 groups, dim3 joins, size_t lds, hipStream_t st, const WideArgs& a) {
+  hipLaunchKernelGGL((wide_fwd_kernel<HD, D, true, true>), groups, dim3(256), lds, st, a);
+  hipLaunchKernelGGL((wide_join_kernel<HD, D>), joins, dim3(256), 0, st, a);
+}
+template <bool D>
+static void wide_split_launch(const DenseAttnCall& c, dim3 groups, dim3 joins, size_t lds, hipStream_t st, const WideArgs& a) {
+  if (c.head_dim == 16) wide_split_hd<D, 16>(c, groups, joins, lds, st, a);
+  else if (c.head_dim == 24) wide_split_hd<D, 24>(c, groups, joins, lds, st, a);
+  else if (c.head_dim == 32) wide_split_hd<D, 32>(c, groups, joins, lds, st, a);
+  else wide_split_hd<D, 64>(c, groups, joins, lds, st, a);
+}
+
 int wide_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
   WidePrep w{};
   w.total_k = c.total_k; w.heads = c.heads; w.tk_tiles = r.tk_tiles;
@@ -989,6 +1069,16 @@ int wide_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hip
   WideArgs a = wide_rel_args(c, r);
   a.knorm = r.knorm; a.tk_tiles = r.tk_tiles;
   a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
+  if (r.split.keys) {
+    a.split = r.split;
+    const dim3 groups((unsigned)(r.split.most * c.heads)), joins((unsigned)(((size_t)c.total_q * c.heads + 3) / 4));
+    ESA_TIMED(esa_profile::kAttnFwd, st, {
+      if (c.dropout) wide_split_launch<true>(c, groups, joins, r.bias.stride * sizeof(float), st, a);
+      else wide_split_launch<false>(c, groups, joins, r.bias.stride * sizeof(float), st, a);
+    });
+    ESA_LAUNCH_CHECK();
+    return ESA_OK;
+  }
   const dim3 grid(wide_grid(c.total_q, c.nseg, c.heads));
   ESA_TIMED(esa_profile::kAttnFwd, st,
             ESA_WIDE_REL_LAUNCH(wide_fwd_kernel, c.head_dim, c.dropout, grid, r.bias.stride * sizeof(float), st, a));

@@ -236,14 +236,20 @@ __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const NormArgs a) {
   }
 }
 
-// dw[n][d] = the sum of part[block][n][d]: 32 columns a block, its 32 rows of threads one after another.
+// dw[n][d] = the sum of part[block][n][d]: 32 columns a block, its 32 rows of threads one after another.  A thread's
+// loads go out eight at a time: one by one the launch took 22 us for 2,048 blocks.
 __global__ __launch_bounds__(1024) void qk_norm_reduce_kernel(const float* __restrict__ part, int blocks, int hd,
                                                               float* __restrict__ dwq, float* __restrict__ dwk) {
   __shared__ float s[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x, cols = 2 * hd;
   float sum = 0.f;
-  if (c < cols)
-    for (int i = y; i < blocks; i += 32) sum += part[(size_t)i * cols + c];
+  for (int i0 = y; i0 < blocks; i0 += 8 * 32) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = i0 + 32 * j < blocks && c < cols ? part[(size_t)(i0 + 32 * j) * cols + c] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[j];
+  }
   s[y][x] = sum;
   __syncthreads();
   if (y || c >= cols) return;

@@ -22,8 +22,16 @@ __global__ __launch_bounds__(kReduceCols* kReduceRows) void rel_reduce_kernel(co
   const int x = threadIdx.x % kReduceCols, y = threadIdx.x / kReduceCols;
   const int cols = heads * buckets, c = blockIdx.x * kReduceCols + x, n = *count;
   float sum = 0.f;
-  if (c < cols)
-    for (int i = y; i < n; i += kReduceRows) sum += part[(size_t)i * cols + c];
+  for (int i0 = y; i0 < n; i0 += 8 * kReduceRows) {   // eight loads in flight
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + kReduceRows * j;
+      v[j] = i < n && c < cols ? part[(size_t)i * cols + c] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[j];
+  }
   s[y][x] = sum;
   __syncthreads();
   if (y || c >= cols) return;
@@ -39,8 +47,24 @@ size_t groups_most(int total, int batch) {
   return (size_t)(total + kGroupTok - 1) / kGroupTok + (size_t)std::min(batch, total) + 1;
 }
 
-struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, line, top, ranges, knorm, rows, part, total; };
-Layout layout(int batch, int total_q, int total_k, int heads, int buckets, int reach, int dtype, bool backward) {
+// The bf16 forward of few queries (at most 32 a segment on average) over many keys (512 and more): with a block per
+// segment and head at most kSplitMaxSegments blocks walk all of a segment's keys, one of their waves at work.  Cut so
+// that about 2,048 blocks have `keys` each, 16 protein graphs (68,000 keys, 16 heads of 32), three queries each, take
+// 14 us and 7 to join them instead of 31.
+int split_keys(int batch, int total_q, int total_k, int heads, int dtype, bool backward) {
+  if (backward || dtype != ESA_BF16 || total_q == 0 || total_q > (long long)kSplitRows * batch || batch > kSplitMaxSegments ||
+      (long long)batch * heads >= 2048 || total_k < 512LL * batch)
+    return 0;
+  const long long want = (long long)total_k * heads / 2048;
+  return (int)std::max(128LL, (want + 127) / 128 * 128);
+}
+// A segment's groups: of 32 queries, or of `keys` keys.
+size_t split_most(int batch, int total_q, int total_k, int keys) {
+  return (size_t)(total_q + kSplitRows - 1) / kSplitRows + (size_t)(total_k + keys - 1) / keys + 2 * (size_t)batch;
+}
+
+struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, line, top, ranges, knorm, rows, part, where, acc, ml, total; };
+Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int buckets, int reach, int dtype, bool backward) {
   Layout w{};
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -49,7 +73,9 @@ Layout layout(int batch, int total_q, int total_k, int heads, int buckets, int r
     return at;
   };
   const int stride = 2 * (reach + kRelPad) + 1;
-  const size_t gq = groups_most(total_q, batch), gk = groups_most(total_k, batch);
+  const int split = split_keys(batch, total_q, total_k, heads, dtype, backward);
+  const size_t gk = groups_most(total_k, batch);
+  const size_t gq = split ? split_most(batch, total_q, total_k, split) : groups_most(total_q, batch);
   w.counts = take(8);
   w.plan_q = take(gq * sizeof(int4));
   w.shift_q = take(gq * sizeof(int));
@@ -62,7 +88,13 @@ Layout layout(int batch, int total_q, int total_k, int heads, int buckets, int r
     w.rows = take((size_t)heads * tiles32(total_q) * kTile * sizeof(float2));
     w.part = take(gq * heads * buckets * sizeof(float));
   } else if (dtype == ESA_BF16) {
-    w.knorm = take((size_t)heads * tiles32(total_k) * sizeof(float));
+    if (!split) w.knorm = take((size_t)heads * tiles32(total_k) * sizeof(float));
+    if (split) {
+      const size_t rows = gq * kWaves * heads * kSplitRows;
+      w.where = take((size_t)total_q * sizeof(int4));
+      w.acc = take(rows * head_dim * sizeof(float));
+      w.ml = take(rows * sizeof(float2));
+    }
   }
   w.total = off;
   return w;
@@ -113,8 +145,15 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
     r.shift_k = reinterpret_cast<int*>(at(w.shift_k));
     r.rows = reinterpret_cast<float2*>(at(w.rows));
   } else if (dtype == ESA_BF16) {
-    r.knorm = reinterpret_cast<float*>(at(w.knorm));
-    r.tk_tiles = tiles32(c.total_k);
+    if ((r.split.keys = split_keys(c.nseg, c.total_q, c.total_k, c.heads, dtype, false))) {
+      r.split.most = (int)split_most(c.nseg, c.total_q, c.total_k, r.split.keys);
+      r.split.where = reinterpret_cast<int4*>(at(w.where));
+      r.split.acc = reinterpret_cast<float*>(at(w.acc));
+      r.split.ml = reinterpret_cast<float2*>(at(w.ml));
+    } else {
+      r.knorm = reinterpret_cast<float*>(at(w.knorm));
+      r.tk_tiles = tiles32(c.total_k);
+    }
   }
   p.cu_q = c.cu_q; p.cu_k = c.cu_k; p.q_start = q_start; p.nseg = c.nseg;
   p.total_q = c.total_q; p.total_k = c.total_k; p.heads = c.heads;
@@ -139,7 +178,9 @@ int esa_rel_attn_workspace_size(int batch, int total_q, int total_k, int heads, 
   if (!bytes) return ESA_ERR_NULL;
   const int rc = check(batch, total_q, total_k, heads, head_dim, dtype, num_buckets, bucket_starts, num_starts);
   if (rc) return rc;
-  *bytes = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, backward != 0).total;
+  *bytes = layout(batch, total_q, total_k, heads, head_dim, num_buckets, reach_of(bucket_starts, num_starts), dtype,
+                  backward != 0)
+               .total;
   return ESA_OK;
 }
 
@@ -158,7 +199,7 @@ int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* ta
     return ESA_ERR_NULL;
   if (off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(workspace))
     return ESA_ERR_ALIGN;
-  const Layout w = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, false);
+  const Layout w = layout(batch, total_q, total_k, heads, head_dim, num_buckets, reach_of(bucket_starts, num_starts), dtype, false);
   if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
   DenseAttnCall c{};
   c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;
@@ -190,7 +231,7 @@ int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void*
   if (off_boundary(dout) || off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(dq) ||
       off_boundary(dk) || off_boundary(dv) || off_boundary(workspace))
     return ESA_ERR_ALIGN;
-  const Layout w = layout(batch, total_q, total_k, heads, num_buckets, reach_of(bucket_starts, num_starts), dtype, true);
+  const Layout w = layout(batch, total_q, total_k, heads, head_dim, num_buckets, reach_of(bucket_starts, num_starts), dtype, true);
   if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
   DenseAttnCall c{};
   c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;

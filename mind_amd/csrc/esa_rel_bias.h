@@ -40,6 +40,25 @@ struct RelBias {
   float* part;              // dQ pass: [groups][heads][buckets]
 };
 
+// Few queries over many keys (bf16 forward): a group is 32 queries of one
+// segment and `keys` of its keys, one block and head each; the block's four
+// waves take every fourth tile of 32 keys for the same queries, and each leaves
+// its unnormalised output, maximum and sum.  One more launch joins them.
+struct RelSplit {
+  int keys;        // keys of a group, a multiple of 128; 0: not split
+  int most;        // groups at most
+  int4* where;     // [total_q]: a query's first group, how many it has, its row in them (no groups: in no segment)
+  float* acc;      // [groups][4][heads][32][head_dim]
+  float2* ml;      // [groups][4][heads][32] maximum (powers of two) and sum
+};
+constexpr int kSplitRows = 32;
+constexpr int kSplitMaxSegments = 2048;
+// Groups of a segment: its keys are cut where its queries fit one group.
+DEVI int2 split_groups(int queries, int keys, int per) {
+  const int ng = (queries + kSplitRows - 1) / kSplitRows;
+  return make_int2(ng, ng == 1 ? max(1, (keys + per - 1) / per) : 1);
+}
+
 // What a call's attention passes read besides its tensors.
 struct RelPass {
   RelBias bias;
@@ -48,6 +67,7 @@ struct RelPass {
   int* shift_q; int* shift_k;       // per group: d = key token - query token - shift
   float* knorm; int tk_tiles;       // bf16 forward: max |k| per (head, 32-key tile)
   float2* rows; int tq_pad;         // backward: row statistics [heads][tq_pad]
+  RelSplit split;                   // bf16 forward of few queries
 };
 
 // The preparation: plans, bias lines and the rows of tokens in no segment.
@@ -238,12 +258,68 @@ DEVI int rel_bucket(const RelPrep& p, int d) {
   return lo + (p.two_sided && d > 0 ? p.side : 0);
 }
 
+// The groups of a split forward (at most kSplitMaxSegments segments), in order.
+template <class ShiftOf>
+DEVI void split_plan_block(const RelPrep& p, const RelPass& r, int tid, ShiftOf shift_of) {
+  constexpr int PER = kSplitMaxSegments / 256;
+  __shared__ int first[kSplitMaxSegments + 1];
+  __shared__ int part[256];
+  int loc[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = tid * PER + i;
+    loc[i] = sum;
+    if (s < p.nseg) {
+      const int2 n = split_groups(max(p.cu_q[s + 1] - p.cu_q[s], 0), p.cu_k[s + 1] - p.cu_k[s], r.split.keys);
+      sum += n.x * n.y;
+    }
+  }
+  part[tid] = sum;
+  __syncthreads();
+  for (int off = 1; off < 256; off <<= 1) {
+    const int add = tid >= off ? part[tid - off] : 0;
+    __syncthreads();
+    part[tid] += add;
+    __syncthreads();
+  }
+  const int base = part[tid] - sum;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = tid * PER + i;
+    first[s] = base + loc[i];
+  }
+  if (tid == 255) {
+    first[kSplitMaxSegments] = part[255];
+    *r.count_q = part[255];
+  }
+  __syncthreads();
+  for (int e = tid; e < part[255]; e += 256) {
+    int lo = 0, hi = p.nseg;   // the last segment that begins at or before e: it is not empty
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= e) lo = mid; else hi = mid;
+    }
+    const int qb = p.cu_q[lo], qe = p.cu_q[lo + 1], kb = p.cu_k[lo], ke = max(p.cu_k[lo + 1], kb);
+    const int2 n = split_groups(qe - qb, ke - kb, r.split.keys);
+    const int g = (e - first[lo]) / n.y, c = (e - first[lo]) % n.y, q0 = qb + g * kSplitRows;
+    const int k0 = n.y == 1 ? kb : kb + c * r.split.keys;
+    r.plan_q[e] = make_int4(q0, min(q0 + kSplitRows, qe), k0, n.y == 1 ? ke : min(k0 + r.split.keys, ke));
+    r.shift_q[e] = shift_of(lo);
+    if (c == 0)
+      for (int t = q0; t < min(q0 + kSplitRows, qe); ++t) r.split.where[t] = make_int4(e, n.y, t - q0, 0);
+  }
+}
+
 // Block b of the preparation's rel_prep_blocks (256 threads).
 DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
   auto shift_of = [&](int s) {
     const int start = p.q_start ? min(max(p.q_start[s], -(1 << 30)), 1 << 30) : 0;
     return p.cu_k[s] - p.cu_q[s] + start;
   };
+  if (b == 0 && r.split.keys) {
+    split_plan_block(p, r, tid, shift_of);
+    return;
+  }
   if (b == 0) {
     seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, r.shift_q, shift_of);
     return;
@@ -300,6 +376,9 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
   clear(p.zero_q, p.cu_q, p.total_q);
   clear(p.zero_k, p.cu_k, p.total_k);
   clear(p.zero_v, p.cu_k, p.total_k);
+  if (r.split.keys)
+    for (int t = min(max(p.cu_q[p.nseg], 0), p.total_q) + b * 256 + tid; t < p.total_q; t += kRelClearBlocks * 256)
+      r.split.where[t] = make_int4(0, 0, 0, 0);
   if (p.lse) {
     const int from = min(max(p.cu_q[p.nseg], 0), p.total_q);
     for (int h = 0; h < p.heads; ++h)

@@ -196,6 +196,8 @@ def test_refused(device):
     for args, kwargs, error in (((g, -1.0), {}, ValueError), ((g, math.nan), {}, ValueError), ((g, 1.0, 1.0), {}, ValueError),
                                 (([torch.zeros(5, device=device, dtype=torch.float16)], 1.0), {}, TypeError),
                                 ((g, 1.0), {"out": []}, ValueError), ((g, 1.0), {"out": [torch.zeros(4, device=device)]}, ValueError),
+                                ((g, 1.0), {"out": [torch.zeros(1, 5, device=device)]}, ValueError),
+                                (([torch.zeros(3)], 1.0), {}, RuntimeError), (([None], 1.0), {}, TypeError),
                                 ((g, 1.0), {"out": [torch.zeros(5, device=device, dtype=torch.bfloat16)]}, TypeError)):
         with pytest.raises(error):
             clip_gradients(*args, **kwargs)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from mind_amd import _lib
-from mind_amd.esa.gradients import _Lists, _separate, clip_gradients, grad_norm
+from mind_amd.esa.gradients import clip_gradients, grad_norm
 from mind_amd.esa.qk_norm import qk_norm_rotary, rotary_frequencies
 
 
@@ -75,31 +75,52 @@ def test_gradient_norm_refuses_host_tensors():
     assert float(grad_norm([])) == 0.0
 
 
-class _Spans(_Lists):
-    def __init__(self, spans):
-        self.n, self._spans = len(spans), np.array(spans, dtype=np.int64).reshape(-1, 2)
-
-    def spans(self):
-        return self._spans[:, 0], self._spans[:, 1]
+def _spans(spans):
+    """(pointers, counts, codes) of float32 tensors over byte spans."""
+    spans = np.array(spans, dtype=np.int64).reshape(-1, 2)
+    return spans[:, 0].tobytes(), ((spans[:, 1] - spans[:, 0]) // 4).tobytes(), np.zeros(len(spans), dtype=np.int32).tobytes()
 
 
 def test_separate_against_every_pair():
-    rng = np.random.default_rng(0)
+    separate, rng = _lib.tensors().separate, np.random.default_rng(0)
     for trial in range(2000):
         n = int(rng.integers(1, 5))
-        first = rng.integers(0, 24, size=(2, n)) * 2
-        size = rng.integers(0, 5, size=(2, n)) * 2
+        first = rng.integers(0, 24, size=(2, n)) * 4
+        size = rng.integers(0, 5, size=(2, n)) * 4
         if trial % 3 == 0:
             first[1], size[1] = first[0], size[0]
-        dst, src = (_Spans([(f, f + s) for f, s in zip(first[i], size[i])]) for i in (0, 1))
+        d, s = ([(int(f), int(f + z)) for f, z in zip(first[i], size[i])] for i in (0, 1))
 
         def shares(a, b):
             return max(a[0], b[0]) < min(a[1], b[1])
-        d, s = dst._spans.tolist(), src._spans.tolist()
         apart = not any(shares(d[i], d[j]) for i in range(n) for j in range(i))
-        assert _separate(dst, dst) == apart
+        assert separate(_spans(d), None) == apart
         want = apart and not any(shares(d[i], s[j]) and not (i == j and d[i] == s[j]) for i in range(n) for j in range(n))
-        assert _separate(dst, src) == want
+        assert separate(_spans(d), _spans(s)) == want
+
+
+def test_describe():
+    describe = _lib.tensors().describe
+    a, b = torch.zeros(3, 5), torch.zeros(8, dtype=torch.bfloat16)
+    ptrs, counts, codes, device, contiguous = describe([a, b])
+    assert np.frombuffer(ptrs, np.int64).tolist() == [a.data_ptr(), b.data_ptr()] and device == -1 and contiguous
+    assert np.frombuffer(counts, np.int64).tolist() == [15, 8] and np.frombuffer(codes, np.int32).tolist() == [0, 1]
+    assert describe([a.t()])[4] is False and describe([])[0] == b""
+    for bad in ([a, 3], (a,), [a.double()], [a.to_sparse()], [None]):
+        with pytest.raises(TypeError):
+            describe(bad)
+    misfit = _lib.tensors().misfit
+    assert misfit([a, b], [a + 1, b.clone()]) is None and misfit([b], [b.float()]) is None
+    assert misfit([a], [a.t()]) == misfit([a], [a, b]) == misfit([a], [a.view(-1)]) == "shapes"
+    assert misfit([a], [a.bfloat16()]) == misfit([b], [b.half()]) == "dtypes"
+    with pytest.raises(TypeError):
+        misfit([a], [3])
+    version = a._version
+    _lib.tensors().changed([a, torch.nn.Parameter(b)])
+    assert a._version == version + 1
+    with torch.inference_mode():
+        inside = torch.zeros(2)
+    _lib.tensors().changed([inside])
 
 
 def test_gradient_entry_points_refuse_before_launch():
@@ -118,11 +139,14 @@ def test_gradient_entry_points_refuse_before_launch():
     assert norm(ptrs=(18,)) == -6 and norm(ptrs=(17,), codes=(1,)) == -6 and norm(out=None) == -1 and norm(ws=None) == -1
     assert norm(nbytes=4) == -4
     p, c, d = lists()
-    assert lib.esa_grad_norm_workspace_size(1, c, ctypes.byref(n)) == 0 and n.value == 8
-    assert lib.esa_grad_norm_workspace_size(1, None, ctypes.byref(n)) == -1
+    assert lib.esa_grad_workspace_size(1, c, 0, ctypes.byref(n)) == 0 and n.value >= 8
+    assert lib.esa_grad_workspace_size(1, None, 0, ctypes.byref(n)) == -1
+    assert lib.esa_grad_workspace_size(1, (ctypes.c_longlong * 1)(-3), 1, ctypes.byref(n)) == -2
 
-    def clip(out=(16,), out_codes=(0,), max_norm=1.0, norm_at=16, **kw):
+    def clip(out=(16,), out_codes=(0,), max_norm=1.0, norm_at=16, ws=16, nbytes=1 << 20, **kw):
         p, c, d = lists(**kw)
-        return lib.esa_grad_clip(1, p, (ctypes.c_void_p * 1)(*out), c, d, (ctypes.c_int * 1)(*out_codes), max_norm, norm_at, None)
+        return lib.esa_grad_clip(1, p, (ctypes.c_void_p * 1)(*out), c, d, (ctypes.c_int * 1)(*out_codes), 0, max_norm, norm_at,
+                                 ws, nbytes, None)
+    assert clip(ws=None) == -1 and clip(ws=12) == -6 and clip(nbytes=16) == -4
     assert clip(out=(None,)) == -1 and clip(out=(18,)) == -6 and clip(out_codes=(1,)) == -5 and clip(norm_at=None) == -1
     assert clip(max_norm=-1.0) == -2 and clip(max_norm=float("nan")) == -2
