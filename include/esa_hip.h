@@ -544,9 +544,12 @@ ESA_API int esa_weight_grad(long long rows, int n, const void* const* g, const v
 /* as +-1e4.  A query without a key gets output 0 and lse -inf, and so does a */
 /* token in no segment.  Tensors, dtypes, head dims, dropout and lse are      */
 /* those of esa_varlen_attn_fwd, but up to 2^28 - 1 tokens of any row size.   */
+/* out_low [total_q, heads, head_dim] bf16 or null, for bf16 calls: what the  */
+/* rounding of out left over; given to the backward, its row statistic D =    */
+/* sum(dout (out + out_low)) has no rounding of the output (2^-8 of a term    */
+/* at most without it).  ESA_F32 calls neither write nor read it.             */
 /* dtable [num_buckets, heads] fp32: sums of dS in a fixed order              */
-/* (deterministic; for bf16 calls their row statistic comes from the rounded  */
-/* output, relative error about 2^-10).  Workspace size from the query.       */
+/* (deterministic).  Workspace size from the query.                           */
 /* ------------------------------------------------------------------------ */
 ESA_API int esa_rel_attn_workspace_size(int batch, int total_q, int total_k, int heads, int head_dim,
                    int dtype, int num_buckets, const int* bucket_starts, int num_starts,
@@ -556,10 +559,10 @@ ESA_API int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const 
                    const int* q_start, const int* cu_seqlens_q, const int* cu_seqlens_k,
                    int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
                    float softmax_scale, float dropout_p, unsigned long long dropout_seed,
-                   void* out, float* softmax_lse, void* workspace, size_t workspace_bytes,
-                   void* stream);
+                   void* out, void* out_low, float* softmax_lse, void* workspace,
+                   size_t workspace_bytes, void* stream);
 ESA_API int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
-                   const void* out, const float* softmax_lse, const void* table,
+                   const void* out, const void* out_low, const float* softmax_lse, const void* table,
                    int table_dtype, int num_buckets, const int* bucket_starts, int num_starts,
                    const int* q_start, const int* cu_seqlens_q, const int* cu_seqlens_k,
                    int batch, int total_q, int total_k, int heads, int head_dim, int dtype,

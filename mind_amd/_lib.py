@@ -124,14 +124,14 @@ _PROTOS = {
     "esa_rel_attn_workspace_size": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                              ctypes.POINTER(_c_int), _c_int, _c_int, ctypes.POINTER(_c_sz)]),
     # q k v | table dtype buckets starts n_starts q_start | cu_q cu_k batch tq tk heads hd dtype | scale dropout_p seed |
-    # out lse ws bytes stream
+    # out out_low lse ws bytes stream
     "esa_rel_attn_fwd": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int, _vp, _vp, _vp,
-                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp, _vp,
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp, _vp, _vp,
                                   _c_sz, _vp]),
-    # dout q k v out lse | as the forward | dq dk dv dtable ws bytes stream
-    "esa_rel_attn_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int, _vp,
-                                  _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp, _vp,
-                                  _vp, _vp, _vp, _c_sz, _vp]),
+    # dout q k v out out_low lse | as the forward | dq dk dv dtable ws bytes stream
+    "esa_rel_attn_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, ctypes.POINTER(_c_int), _c_int,
+                                  _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f, _c_f, _c_u64, _vp,
+                                  _vp, _vp, _vp, _vp, _c_sz, _vp]),
     # q k strides[4] total hq hk hd dtype | wq wk positions bytes frequencies rotary interleaved eps | q_out k_out stream
     "esa_qk_norm_fwd": (_c_int, [_vp, _vp, ctypes.POINTER(ctypes.c_longlong), _c_int, _c_int, _c_int, _c_int, _c_int, _vp,
                                  _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_f, _vp, _vp, _vp]),

@@ -12,7 +12,9 @@ struct DenseAttnCall {
   int total_q, total_k, heads, head_dim;
   float scale;
   void* out; float* lse;                             // forward outputs
+  void* out_low;                                     // with a relative position bias: what out's rounding left, or null
   const void* out_in; const void* dout; const float* lse_in;   // backward inputs
+  const void* out_low_in;                            // out_low of the forward, or null
   void* dq; void* dk; void* dv;                      // backward outputs
   DropoutCfg drop; bool dropout;                     // attention dropout (esa_common.h) when `dropout`
 };

@@ -59,6 +59,7 @@ struct DenseArgs {
   float c, scale;              // c = scale * log2(e)
   bf16* o; float* lse_out; bf16* dq; bf16* dk; bf16* dv;
   RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
+  const bf16* low; bf16* low_out;  // BIAS: out's rounding residue, or null
 };
 
 // ------------------------------------------------------------------ block mapping
@@ -342,6 +343,13 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(ESA_DENSE_WAVES_FWD) void dense
     if (!valid[u]) continue;
     const float l = acc[u][8];   // a ones row of [V^T; 1] P^T: the softmax row sum
     store_rows8(a.o + ((size_t)t[u] * H + head) * kHd, acc[u], l > 0.f ? 1.f / l : 0.f, half);
+    if (BIAS && a.low_out) {   // what the rounding of the output leaves, for the backward's D
+      const float mul = l > 0.f ? 1.f / l : 0.f;
+      f32x16 rest;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) rest[r] = acc[u][r] * mul - (float)(bf16)(acc[u][r] * mul);
+      store_rows8(a.low_out + ((size_t)t[u] * H + head) * kHd, rest, 1.f, half);
+    }
     if (half == 0)
       a.lse_out[(size_t)head * a.total_q + t[u]] = l > 0.f ? (m_run[u] + fast_log2(l)) * kLn2 : -INFINITY;
   }
@@ -397,9 +405,18 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DQ) 
       for (int e = 0; e < 8; ++e) dsum = fmaf((float)d0[e], (float)p0[e], dsum);
 #pragma unroll
       for (int e = 0; e < 8; ++e) dsum = fmaf((float)d1[e], (float)p1[e], dsum);
+      if (BIAS && a.low) {
+        const bf16x8 l0 = *reinterpret_cast<const bf16x8*>(a.low + row);
+        const bf16x8 l1 = *reinterpret_cast<const bf16x8*>(a.low + row + 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dsum = fmaf((float)d0[e], (float)l0[e], dsum);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dsum = fmaf((float)d1[e], (float)l1[e], dsum);
+      }
       qs[u][qb] = scaled_half(*reinterpret_cast<const bf16x8*>(a.q + row + 8 * (grp & 1)), a.c, grp >= 2);
       ob[u][qb] = *reinterpret_cast<const bf16x4*>(a.dout + row + 4 * grp);
       const float lq = a.lse[(size_t)head * a.total_q + tc];
+      if (BIAS && lq == -INFINITY) dsum = 0.f;   // no key: a split forward left `low` unwritten
       // seed of S': -LSE2; with a bias the lanes past the segment's end have none (their dS is summed by distance)
       cl[u][qb] = splat4(lq == -INFINITY || (BIAS && t >= g.y) ? -INFINITY : -lq * kLog2e);
       cd[u][qb] = splat4(-dsum);                                        // seed of dP: -D
@@ -429,18 +446,14 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DQ) 
   int base = 0;
   f32x4 far_seed[2];   // -LSE2 plus that value
   f32x4 kept[2][4];    // a near stage's dS by query and key block
-  // Far stages: dS summed over the keys by a product with ones, on the matrix pipe instead of an addition per score (of
-  // the bf16 dS that the dQ product takes: 2^-9 of a term, as the rounding of the row statistic).  A stage on the
-  // other side of the window takes the sum so far to its bucket.
-  f32x4 far_acc[2] = {f32x4{}, f32x4{}};
+  // Far stages: their dS in one sum per lane, in 32 bits (a product with ones on the matrix pipe would take them rounded
+  // to bf16 and was no faster).  A stage on the other side of the window takes the sum so far to its bucket.
+  float far_sum = 0.f;
   bool far_side = false;
   auto far_done = [&]() {
-    if (grp == 0) (far_side ? sums.hi : sums.lo) += far_acc[0][0] + far_acc[1][0];   // every row of a product is the sum
-    far_acc[0] = far_acc[1] = f32x4{};
+    (far_side ? sums.hi : sums.lo) += far_sum;
+    far_sum = 0.f;
   };
-  bf16x8 ones;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
 
   f32x4 acc[T][2];
 #pragma unroll
@@ -505,7 +518,8 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DQ) 
             kept[qb][2 * j] = ds[0];
             kept[qb][2 * j + 1] = ds[1];
           } else {
-            far_acc[qb] = mfma16k32(ones, cvt4x2(ds[0], ds[1]), far_acc[qb]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) far_sum += ds[0][e] + ds[1][e];
           }
         }
         acc[u][qb] = mfma16k32(kt, cvt4x2(ds[0], ds[1]), acc[u][qb]);
@@ -911,6 +925,7 @@ int dense_rel_fwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream
   DenseArgs a = dense_rel_args(c, r);
   a.knorm = r.knorm; a.tk_tiles = r.tk_tiles;
   a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
+  a.low_out = static_cast<bf16*>(c.out_low);
   ESA_TIMED(esa_profile::kAttnFwd, st,
             hipLaunchKernelGGL(dense_fwd_kernel<true>, dim3(group_grid(c.total_q, c.nseg, c.heads, kFwdGroup)), dim3(256),
                                r.bias.stride * sizeof(float), st, a));
@@ -928,6 +943,7 @@ int dense_rel_bwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream
   DenseArgs a = dense_rel_args(c, r);
   a.out = static_cast<const bf16*>(c.out_in); a.dout = static_cast<const bf16*>(c.dout);
   a.lse = c.lse_in; a.aux = r.rows; a.aux_out = r.rows;
+  a.low = static_cast<const bf16*>(c.out_low_in);
   a.dq = static_cast<bf16*>(c.dq); a.dk = static_cast<bf16*>(c.dk); a.dv = static_cast<bf16*>(c.dv);
   if (c.total_q > 0)
     ESA_TIMED(esa_profile::kAttnBwdDq, st,

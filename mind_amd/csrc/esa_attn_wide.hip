@@ -82,6 +82,7 @@ struct WideArgs {
   bf16* o; float* lse_out; bf16* dq; bf16* dk; bf16* dv;
   RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
   RelSplit split;                  // SPLIT: where the waves' parts go
+  const bf16* low; bf16* low_out;  // BIAS: out's rounding residue, or null
 };
 
 // LDS position of staged token t in octet o of an NO-octet layout.  The
@@ -490,6 +491,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 &&
     return;
   }
   store_acc<HD>(a.o + ((size_t)t * H + head) * HD, acc, l > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / l : 0.f, h);
+  if (BIAS && a.low_out) {   // what the rounding of the output leaves, for the backward's D
+    const float mul = l > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / l : 0.f;
+    f32x16 rest[NM];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rest[m][r] = acc[m][r] * mul - (float)(bf16)(acc[m][r] * mul);
+    store_acc<HD>(a.low_out + ((size_t)t * H + head) * HD, rest, 1.f, h);
+  }
   if (h == 0)
     a.lse_out[(size_t)head * a.total_q + t] =
         l > 0.f ? ((BIAS ? m_run : a.c * m_run) + fast_log2(l)) * kLn2 : -INFINITY;
@@ -540,7 +550,12 @@ __global__ __launch_bounds__(256) void wide_join_kernel(const WideArgs a) {
   }
   if (SIDE == 2) out += __shfl_xor(out, 32);
   const float mul = sum > 0.f ? (DROP ? a.drop.inv_keep : 1.f) / sum : sum != sum ? sum : 0.f;
-  if (side == 0 && d < HD) a.o[((size_t)t * a.heads + head) * HD + d] = (bf16)(out * mul);
+  if (side == 0 && d < HD) {
+    const size_t to = ((size_t)t * a.heads + head) * HD + d;
+    const bf16 x = (bf16)(out * mul);
+    a.o[to] = x;
+    if (a.low_out) a.low_out[to] = (bf16)(out * mul - (float)x);
+  }
   if (lane == 0)
     a.lse_out[(size_t)head * a.total_q + t] = sum > 0.f ? (all + fast_log2(sum)) * kLn2 : sum != sum ? sum : -INFINITY;
 }
@@ -575,10 +590,16 @@ void wide_dq_kernel(const WideArgs a) {
     const bf16x8 o = row_op<HD>(a.out + row, 2 * c + h);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dsum = fmaf((float)gop[c][e], (float)o[e], dsum);
+    if (BIAS && a.low) {
+      const bf16x8 rest = row_op<HD>(a.low + row, 2 * c + h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dsum = fmaf((float)gop[c][e], (float)rest[e], dsum);
+    }
   }
   wide_zero_pad<HD>(sK[0], sK[1], sV[0], sV[1], tid);
   dsum += __shfl_xor(dsum, 32);
   const float lq = a.lse[(size_t)head * a.total_q + (valid ? t : g.x)];
+  if (BIAS && lq == -INFINITY) dsum = 0.f;   // no key: a split forward left `low` unwritten
   // rows without keys, and with a bias the lanes past the segment's end (their dS is summed by distance): P = 0
   const float lse2 = lq == -INFINITY || (BIAS && !valid) ? INFINITY : lq * kLog2e;
   if (valid && h == 0)
@@ -1069,6 +1090,7 @@ int wide_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hip
   WideArgs a = wide_rel_args(c, r);
   a.knorm = r.knorm; a.tk_tiles = r.tk_tiles;
   a.o = static_cast<bf16*>(c.out); a.lse_out = c.lse;
+  a.low_out = static_cast<bf16*>(c.out_low);
   if (r.split.keys) {
     a.split = r.split;
     const dim3 groups((unsigned)(r.split.most * c.heads)), joins((unsigned)(((size_t)c.total_q * c.heads + 3) / 4));
@@ -1094,6 +1116,7 @@ int wide_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hip
   WideArgs a = wide_rel_args(c, r);
   a.out = static_cast<const bf16*>(c.out_in); a.dout = static_cast<const bf16*>(c.dout);
   a.lse = c.lse_in; a.aux = r.rows;
+  a.low = static_cast<const bf16*>(c.out_low_in);
   a.dq = static_cast<bf16*>(c.dq); a.dk = static_cast<bf16*>(c.dk); a.dv = static_cast<bf16*>(c.dv);
   const size_t line = r.bias.stride * sizeof(float);
   if (c.total_q > 0)

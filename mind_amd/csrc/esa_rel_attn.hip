@@ -187,8 +187,8 @@ int esa_rel_attn_workspace_size(int batch, int total_q, int total_k, int heads, 
 int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, int table_dtype, int num_buckets,
                      const int* bucket_starts, int num_starts, const int* q_start, const int* cu_seqlens_q,
                      const int* cu_seqlens_k, int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
-                     float softmax_scale, float dropout_p, unsigned long long dropout_seed, void* out, float* softmax_lse,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+                     float softmax_scale, float dropout_p, unsigned long long dropout_seed, void* out, void* out_low,
+                     float* softmax_lse, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check(batch, total_q, total_k, heads, head_dim, dtype, num_buckets, bucket_starts, num_starts);
   if (rc) return rc;
   if (table_dtype != ESA_BF16 && table_dtype != ESA_F32) return ESA_ERR_DTYPE;
@@ -197,14 +197,15 @@ int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* ta
   if (total_q == 0) return ESA_OK;
   if (!table || !cu_seqlens_q || !cu_seqlens_k || !workspace || !q || !out || !softmax_lse || (total_k > 0 && (!k || !v)))
     return ESA_ERR_NULL;
-  if (off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(workspace))
+  if (off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(out_low) ||
+      off_boundary(workspace))
     return ESA_ERR_ALIGN;
   const Layout w = layout(batch, total_q, total_k, heads, head_dim, num_buckets, reach_of(bucket_starts, num_starts), dtype, false);
   if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
   DenseAttnCall c{};
   c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;
   c.total_q = total_q; c.total_k = total_k; c.heads = heads; c.head_dim = head_dim; c.scale = softmax_scale;
-  c.out = out; c.lse = softmax_lse;
+  c.out = out; c.out_low = out_low; c.lse = softmax_lse;
   c.drop = make_dropout(dropout_p, dropout_seed, heads); c.dropout = dropout_p > 0.f;
   RelPass r{};
   RelPrep p{};
@@ -214,7 +215,7 @@ int esa_rel_attn_fwd(const void* q, const void* k, const void* v, const void* ta
   return dtype == ESA_BF16 ? dense_rel_fwd(c, r, p, st) : f32_rel_fwd(c, r, p, st);
 }
 
-int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* out_low,
                      const float* softmax_lse, const void* table, int table_dtype, int num_buckets,
                      const int* bucket_starts, int num_starts, const int* q_start, const int* cu_seqlens_q,
                      const int* cu_seqlens_k, int batch, int total_q, int total_k, int heads, int head_dim, int dtype,
@@ -228,15 +229,15 @@ int esa_rel_attn_bwd(const void* dout, const void* q, const void* k, const void*
   if (!table || !dtable || !cu_seqlens_q || !cu_seqlens_k || !workspace ||
       (total_q > 0 && (!dout || !q || !out || !softmax_lse || !dq)) || (total_k > 0 && (!k || !v || !dk || !dv)))
     return ESA_ERR_NULL;
-  if (off_boundary(dout) || off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) || off_boundary(dq) ||
-      off_boundary(dk) || off_boundary(dv) || off_boundary(workspace))
+  if (off_boundary(dout) || off_boundary(q) || off_boundary(k) || off_boundary(v) || off_boundary(out) ||
+      off_boundary(out_low) || off_boundary(dq) || off_boundary(dk) || off_boundary(dv) || off_boundary(workspace))
     return ESA_ERR_ALIGN;
   const Layout w = layout(batch, total_q, total_k, heads, head_dim, num_buckets, reach_of(bucket_starts, num_starts), dtype, true);
   if (workspace_bytes < w.total) return ESA_ERR_WORKSPACE;
   DenseAttnCall c{};
   c.q = q; c.k = k; c.v = v; c.cu_q = cu_seqlens_q; c.cu_k = cu_seqlens_k; c.nseg = batch;
   c.total_q = total_q; c.total_k = total_k; c.heads = heads; c.head_dim = head_dim; c.scale = softmax_scale;
-  c.out_in = out; c.dout = dout; c.lse_in = softmax_lse; c.dq = dq; c.dk = dk; c.dv = dv;
+  c.out_in = out; c.out_low_in = out_low; c.dout = dout; c.lse_in = softmax_lse; c.dq = dq; c.dk = dk; c.dv = dv;
   c.drop = make_dropout(dropout_p, dropout_seed, heads); c.dropout = dropout_p > 0.f;
   RelPass r{};
   RelPrep p{};

@@ -68,6 +68,8 @@ class _RelativeAttention(torch.autograd.Function):
         (tq, heads, hd), tk, batch, dt = q.shape, k.shape[0], cu_q.numel() - 1, _dtype_code(q)
         table = bias.contiguous()
         out = torch.empty_like(q)
+        # what the rounding of out leaves, where a backward may need it: its row statistic is exact then
+        low = torch.empty_like(q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else None
         lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device)
         c_starts = (ctypes.c_int * len(starts))(*starts)
         with _lib.on_device(q):
@@ -75,9 +77,9 @@ class _RelativeAttention(torch.autograd.Function):
             _lib.check(_lib.load().esa_rel_attn_fwd(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), _TABLE[table.dtype], table.shape[0], c_starts,
                 len(starts), _lib.ptr(q_start), cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, heads, hd, dt, scale,
-                dropout_p, seed, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)),
+                dropout_p, seed, out.data_ptr(), _lib.ptr(low), lse.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)),
                 "esa_rel_attn_fwd")
-        ctx.save_for_backward(q, k, v, table, out, lse, cu_q, cu_k, q_start)
+        ctx.save_for_backward(q, k, v, table, out, low, lse, cu_q, cu_k, q_start)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
         ctx.meta = (starts, scale, dropout_p, seed)
@@ -86,7 +88,7 @@ class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
-        q, k, v, table, out, lse, cu_q, cu_k, q_start = ctx.saved_tensors
+        q, k, v, table, out, low, lse, cu_q, cu_k, q_start = ctx.saved_tensors
         if g is None:
             return (None,) * 11
         starts, scale, dropout_p, seed = ctx.meta
@@ -98,8 +100,8 @@ class _RelativeAttention(torch.autograd.Function):
         with _lib.on_device(q):
             ws = _workspace(q.device, batch, tq, tk, heads, hd, dt, table.shape[0], c_starts, True)
             _lib.check(_lib.load().esa_rel_attn_bwd(
-                g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), table.data_ptr(),
-                _TABLE[table.dtype], table.shape[0], c_starts, len(starts), _lib.ptr(q_start), cu_q.data_ptr(),
+                g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(low), lse.data_ptr(),
+                table.data_ptr(), _TABLE[table.dtype], table.shape[0], c_starts, len(starts), _lib.ptr(q_start), cu_q.data_ptr(),
                 cu_k.data_ptr(), batch, tq, tk, heads, hd, dt, scale, dropout_p, seed, dq.data_ptr(), dk.data_ptr(),
                 dv.data_ptr(), dtable.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)), "esa_rel_attn_bwd")
         return dq, dk, dv, dtable.to(table.dtype), None, None, None, None, None, None, None

@@ -77,13 +77,13 @@ def test_entry_points_refuse_before_launch():
     s = (ctypes.c_int * 2)(0, 3)
 
     def fwd(q=16, table=16, tdt=0, scale=0.25, p=0.0, ws=16, nbytes=1 << 24, tq=100):
-        return lib.esa_rel_attn_fwd(q, 16, 16, table, tdt, 4, s, 2, None, 16, 16, 2, tq, 90, 4, 16, bf16, scale, p, 0, 16, 16,
-                                    ws, nbytes, None)
+        return lib.esa_rel_attn_fwd(q, 16, 16, table, tdt, 4, s, 2, None, 16, 16, 2, tq, 90, 4, 16, bf16, scale, p, 0, 16, None,
+                                    16, ws, nbytes, None)
     assert fwd(q=None) == -1 and fwd(table=None) == -1 and fwd(q=8) == -6 and fwd(tdt=3) == -5 and fwd(scale=0.0) == -2
     assert fwd(scale=float("nan")) == -2 and fwd(p=1.0) == -9 and fwd(nbytes=256) == -4 and fwd(ws=None) == -1
     assert fwd(tq=0, q=None) == 0   # no queries: nothing to do
 
-    def bwd(g=16, dtable=16, nbytes=1 << 24):
-        return lib.esa_rel_attn_bwd(g, 16, 16, 16, 16, 16, 16, 0, 4, s, 2, None, 16, 16, 2, 100, 90, 4, 16, bf16, 0.25, 0.0,
+    def bwd(g=16, dtable=16, nbytes=1 << 24, low=None):
+        return lib.esa_rel_attn_bwd(g, 16, 16, 16, 16, low, 16, 16, 0, 4, s, 2, None, 16, 16, 2, 100, 90, 4, 16, bf16, 0.25, 0.0,
                                     0, 16, 16, 16, dtable, 16, nbytes, None)
-    assert bwd(g=None) == -1 and bwd(dtable=None) == -1 and bwd(g=24) == -6 and bwd(nbytes=64) == -4
+    assert bwd(g=None) == -1 and bwd(dtable=None) == -1 and bwd(g=24) == -6 and bwd(low=24) == -6 and bwd(nbytes=64) == -4
