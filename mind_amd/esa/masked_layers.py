@@ -43,6 +43,7 @@ from .mha_flash_varlen import PMAFlashVarlen, SABFlashVarlen
 from .mlp_utils import GatedMLPMulti, SmallMLP
 from .norm_layers import LN
 from .packing import EdgeAdjacency, NodeAdjacency, PackedSets
+from .token_order import OrderedHeads, TokenOrder
 
 
 def get_adj_mask_from_edge_index_edge(edge_index, batch_size, max_items, batch_mapping, xformers_or_torch_attn=None,
@@ -81,7 +82,7 @@ class SABComplete(nn.Module):
                  set_max_items=0, use_bfloat16=True, num_mlp_layers=3, pre_or_post="pre",
                  num_layers_for_residual=0, use_mlp_ln=False, mlp_dropout=0, use_equivariant=False,
                  equivariant_lmax=2, equivariant_num_features=16, equivariant_fusion_method="add",
-                 equivariant_cross_connection=True):
+                 equivariant_cross_connection=True, token_order=None):
         super().__init__()
         _backend_check(xformers_or_torch_attn)
         if use_equivariant:
@@ -106,6 +107,12 @@ class SABComplete(nn.Module):
             self.sab = SABFlashVarlen(dim_in, dim_out, num_heads, dropout)
         else:
             self.sab = SAB(dim_in, dim_out, num_heads, dropout, xformers_or_torch_attn)
+        if token_order is not None:
+            if xformers_or_torch_attn != "hip" or idx not in (0, 1):
+                raise ValueError("token_order is for the \"hip\" backend's encoder layers")
+            if dim_out % num_heads:
+                raise ValueError("Embedding dim is not divisible by nheads")
+            self.sab.mab.order = OrderedHeads(token_order, num_heads, dim_out // num_heads, masked=idx == 1)
         self.norm = LN(dim_in, num_elements=set_max_items if idx != 2 else None)
         self.mlp_type = mlp_type
         if use_mlp:
@@ -116,6 +123,11 @@ class SABComplete(nn.Module):
 
     def forward(self, inp):
         X, edge_index, batch_mapping, max_items, adj_mask = inp[:5]
+        if isinstance(self.sab, SAB) and self.sab.mab.order is not None:
+            if not isinstance(adj_mask, PackedSets):
+                raise TypeError("a block with a token order needs its tokens' EdgeAdjacency / NodeAdjacency descriptor")
+            out = adj_mask.pad(_sab_forward_packed(self, adj_mask.unpad(X), adj_mask))
+            return out, edge_index, batch_mapping, max_items, adj_mask
         X = self.norm(X)
         if isinstance(self.sab, SABFlashVarlen):
             # the reference's seq_lens: node counts per graph, mask dropped (esa/masked_layers.py:422-438)
@@ -155,14 +167,19 @@ def _sab_valid_only(sab: SAB, X: torch.Tensor, tokens: PackedSets) -> torch.Tens
 
 def _packed_mab(mab, xq: torch.Tensor, xk: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor, max_q: int,
                 max_k: int, mask_kwargs: dict, residual: torch.Tensor | None = None,
-                seed: int | None = None) -> torch.Tensor:
+                seed: int | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
     """MAB (esa/mha.py:48-89, V = fc_v(K)) on packed rows: queries xq [Tq, D] and keys xk [Tk, D] grouped by
     cu_q / cu_k -> [Tq, D] (``xk is xq`` for self-attention), plus the block residual when given.  The
-    projections and the fc_o + Mish epilogue run fused (qkv_projection, mab_epilogue)."""
+    projections and the fc_o + Mish epilogue run fused (qkv_projection, mab_epilogue).  ``positions``: each token's
+    index in its graph, for a block with a token order."""
     q, k, v = qkv_projection(mab.fc_q, mab.fc_k, mab.fc_v, xq, xk)
     h, d = mab.num_heads, q.shape[-1]
-    out = varlen_attention(_heads(q, h), _heads(k, h), _heads(v, h), cu_q, cu_k, max_q, max_k,
-                           dropout_p=attn_dropout(mab), dropout_seed=seed, **mask_kwargs)
+    if mab.order is not None:
+        out = mab.order(_heads(q, h), _heads(k, h), _heads(v, h), positions, cu_q, max_q, attn_dropout(mab), seed,
+                        **mask_kwargs)
+    else:
+        out = varlen_attention(_heads(q, h), _heads(k, h), _heads(v, h), cu_q, cu_k, max_q, max_k,
+                               dropout_p=attn_dropout(mab), dropout_seed=seed, **mask_kwargs)
     return mab_epilogue(out.reshape(-1, d).to(q.dtype), mab.fc_o, residual)
 
 
@@ -176,6 +193,8 @@ def _gemm_input_norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
 def _sab_forward_packed(blk: "SABComplete", X: torch.Tensor, tokens: PackedSets) -> torch.Tensor:
     """SABComplete.forward (pre-norm, esa/masked_layers.py:418-483) on packed tokens X [T, D]: the masked
     layers (idx 1) apply the descriptor's mask, the unmasked ones (idx 0) attend over each graph's tokens."""
+    if blk.sab.mab.order is not None:   # the fused block's attention takes its projections as they are
+        return _sab_separate(blk, X, tokens)
     out = sab_block(blk, X, tokens, blk.idx == 1, attn_dropout(blk.sab.mab),
                     lambda b, x, seed: _sab_separate(b, x, tokens, seed))
     return _sab_separate(blk, X, tokens) if out is None else out
@@ -188,9 +207,10 @@ def _sab_separate(blk: "SABComplete", X: torch.Tensor, tokens: PackedSets, seed:
     mask_kwargs = tokens.kernel_mask(padded=False) if blk.idx == 1 else {}
     cu, n = tokens.cu_seqlens, tokens.max_items
     if blk.sab.mab.dim_V == X.shape[-1]:   # the residual add fused into the epilogue
-        out = _packed_mab(blk.sab.mab, x_mm, x_mm, cu, cu, n, n, mask_kwargs, residual=X, seed=seed)
+        out = _packed_mab(blk.sab.mab, x_mm, x_mm, cu, cu, n, n, mask_kwargs, residual=X, seed=seed, positions=tokens.position)
     else:
-        out = blk.proj_1(X) + _packed_mab(blk.sab.mab, x_mm, x_mm, cu, cu, n, n, mask_kwargs, seed=seed)
+        out = blk.proj_1(X) + _packed_mab(blk.sab.mab, x_mm, x_mm, cu, cu, n, n, mask_kwargs, seed=seed,
+                                         positions=tokens.position)
     if blk.use_mlp:
         # out feeds the MLP's LayerNorm and the residual: the pass-through output hands the residual's
         # gradient to the LayerNorm backward, which adds it to its input gradient in the same pass
@@ -286,14 +306,18 @@ class PMAComplete(nn.Module):
 
 
 class ESA(nn.Module):
-    """Edge-set attention encoder + PMA decoder (esa/masked_layers.py:624-936)."""
+    """Edge-set attention encoder + PMA decoder (esa/masked_layers.py:624-936).
+
+    ``token_order`` (a ``TokenOrder``, "hip" backend; no counterpart in the reference): the encoder's layers know each
+    token's index in its graph."""
 
     def __init__(self, num_outputs, dim_output, dim_hidden, num_heads, layer_types, node_or_edge="edge",
                  xformers_or_torch_attn="xformers", pre_or_post="pre", norm_type="LN", sab_dropout=0.0,
                  mab_dropout=0.0, pma_dropout=0.0, residual_dropout=0.0, pma_residual_dropout=0.0, use_mlps=False,
                  mlp_hidden_size=64, num_mlp_layers=2, mlp_type="gated_mlp", mlp_dropout=0.0, use_mlp_ln=False,
                  set_max_items=0, use_bfloat16=True, use_equivariant=False, equivariant_lmax=2,
-                 equivariant_num_features=16, equivariant_fusion_method="add", equivariant_cross_connection=True):
+                 equivariant_num_features=16, equivariant_fusion_method="add", equivariant_cross_connection=True,
+                 token_order: TokenOrder | None = None):
         super().__init__()
         assert len(layer_types) == len(dim_hidden) and len(layer_types) == len(num_heads)
         _backend_check(xformers_or_torch_attn)
@@ -318,11 +342,11 @@ class ESA(nn.Module):
             if lt == "S" and not pma_encountered:
                 encoder.append(SABComplete(d_in, d_out, heads, idx=0, dropout=sab_dropout, node_or_edge=node_or_edge,
                                            xformers_or_torch_attn=xformers_or_torch_attn,
-                                           residual_dropout=residual_dropout, **common))
+                                           residual_dropout=residual_dropout, token_order=token_order, **common))
             if lt == "M" and not pma_encountered:
                 encoder.append(SABComplete(d_in, d_out, heads, idx=1, dropout=mab_dropout, node_or_edge=node_or_edge,
                                            xformers_or_torch_attn=xformers_or_torch_attn,
-                                           residual_dropout=residual_dropout, **common))
+                                           residual_dropout=residual_dropout, token_order=token_order, **common))
             if lt == "P":
                 pma_encountered = True
                 dim_pma = d_in

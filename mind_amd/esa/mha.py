@@ -165,6 +165,7 @@ class MAB(nn.Module):
         self.dim_Q, self.dim_K, self.dim_V = dim_Q, dim_K, dim_V
         self.num_heads = num_heads
         self.dropout_p = dropout_p
+        self.order = None   # an OrderedHeads where the block's tokens have an order (packed "hip" path)
         self.fc_q = nn.Linear(dim_Q, dim_V, bias=True)
         self.fc_k = nn.Linear(dim_K, dim_V, bias=True)
         self.fc_v = nn.Linear(dim_K, dim_V, bias=True)
@@ -177,6 +178,8 @@ class MAB(nn.Module):
     def forward(self, Q, K, adj_mask=None):
         if self.dim_V % self.num_heads:
             raise ValueError("Embedding dim is not divisible by nheads")
+        if self.order is not None:
+            raise RuntimeError("a block with a token order runs through SABComplete on packed tokens")
         p = attn_dropout(self)
         q = self.fc_q(Q)
         v = self.fc_v(K)

@@ -150,3 +150,28 @@ def test_gradient_entry_points_refuse_before_launch():
     assert clip(ws=None) == -1 and clip(ws=12) == -6 and clip(nbytes=16) == -4
     assert clip(out=(None,)) == -1 and clip(out=(18,)) == -6 and clip(out_codes=(1,)) == -5 and clip(norm_at=None) == -1
     assert clip(max_norm=-1.0) == -2 and clip(max_norm=float("nan")) == -2
+
+
+def test_token_order_is_the_packed_encoders():
+    from mind_amd.esa.masked_layers import ESA, SABComplete
+    from mind_amd.esa.token_order import TokenOrder
+    args = (2, 8, [32, 32], [2, 2], ["S", "P"])
+    order = TokenOrder(num_buckets=4, max_distance=10)
+    for backend in ("xformers", "torch", "flash_varlen"):
+        with pytest.raises(ValueError):
+            ESA(*args, xformers_or_torch_attn=backend, token_order=order)
+    with pytest.raises(ValueError):
+        SABComplete(32, 32, 2, 0.0, 2, "LN", xformers_or_torch_attn="hip", token_order=order)   # a decoder layer
+    with pytest.raises(ValueError):
+        SABComplete(32, 32, 3, 0.0, 0, "LN", xformers_or_torch_attn="hip", token_order=order)   # 32 dims in 3 heads
+    with pytest.raises(ValueError):
+        SABComplete(32, 32, 4, 0.0, 0, "LN", xformers_or_torch_attn="hip", token_order=order)   # head dim 8
+    for bad in (TokenOrder(rotary_dim=12), TokenOrder(rotary_dim=24), TokenOrder(num_buckets=5)):
+        with pytest.raises(ValueError):
+            ESA(*args, xformers_or_torch_attn="hip", token_order=bad)
+    m = ESA(*args, xformers_or_torch_attn="hip", token_order=order)
+    x = torch.zeros(1, 4, 32)
+    with pytest.raises(TypeError):
+        m.encoder[0]((x, None, None, 4, None))
+    with pytest.raises(RuntimeError):
+        m.encoder[0].sab(x)
