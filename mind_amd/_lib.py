@@ -191,6 +191,12 @@ def tensors():
     return module
 
 
+@functools.lru_cache(maxsize=None)
+def address(name: str) -> int:
+    """Where an entry point lies, for the host module."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+
+
 def exported_symbols() -> list[str]:
     return list(_PROTOS)
 
@@ -213,6 +219,12 @@ def require_one_device(*tensors: torch.Tensor) -> None:
     for t in tensors[1:]:
         if t.device != first:
             raise EsaError(f"tensors on different devices: {first} and {t.device}")
+
+
+def require_on_one_gpu(*tensors: torch.Tensor | None) -> None:
+    tensors = [t for t in tensors if t is not None]
+    require_gpu(*tensors)
+    require_one_device(*tensors)
 
 
 def on_device(t: torch.Tensor):

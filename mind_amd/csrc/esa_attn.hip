@@ -1355,6 +1355,7 @@ struct AttnF32Args {
   const int* count;         // number of groups
   float* o; float* lse_out; float* dq; float* dk; float* dv;
   RelBias rel; const int* shift;   // BIAS: the relative position bias and the pass's shift per group
+  int group_tok;                   // BIAS: tokens of the plan's groups
 };
 
 // Rows of HD fp32 values (HD = 16, 24, 32 or 64) as float4 chunks.
@@ -1405,12 +1406,16 @@ DEVI bool admissible_f32(int p, int phi, int oi, int2 pn, int2 own) {
 // 90 / 103 / 122 and 103 / 123 / 156 us; 8 heads of 64, dense: 445 / 1054 / 2071
 // -> 221 / 296 / 406 us (93-107 of the 154 TFLOP/s of a large fp32 product).
 constexpr int kF32Stage = 64;
+// By head dim and tokens of a group (kGroupTok, or kFewTok where blocks are few): column blocks per wave, threads.
+constexpr int f32_blocks(int head_dim, int tok) { return head_dim <= 32 && tok == kGroupTok ? 2 : 1; }
+constexpr int f32_threads(int head_dim, int tok) { return 64 * (tok / (16 * f32_blocks(head_dim, tok))); }
 
-template <int HD>
+template <int HD, int TOK = kGroupTok>
 struct F32Tile {
+  static constexpr int kHd = HD;
   static constexpr int NR = (HD + 15) / 16;              // 16-dim chunks of a row
-  static constexpr int QB = HD <= 32 ? 2 : 1;            // column blocks per wave
-  static constexpr int kThreads = 64 * (kGroupTok / (16 * QB));
+  static constexpr int QB = f32_blocks(HD, TOK);         // column blocks per wave
+  static constexpr int kThreads = f32_threads(HD, TOK);
   static constexpr int kStride = 16 * NR + 4;            // floats per staged row
   static constexpr int kPer = kF32Stage * 4 * NR / kThreads;   // 16-byte chunks per thread and staged tensor
   typedef float Rows[kF32Stage][kStride];
@@ -1420,9 +1425,9 @@ DEVI f32x4 mfma16x4f(float a, float b, const f32x4& c) { return __builtin_amdgcn
 
 // The stage's rows of a [T][H][HD] tensor from token t0 on, into registers and from there into LDS; tokens at or
 // past `end` are zeros, or with REPEAT the last row again.
-template <int HD, bool REPEAT = false>
-DEVI void f32_load(f32x4 (&r)[F32Tile<HD>::kPer], const float* src, int end, int H, int head, int t0) {
-  using T = F32Tile<HD>;
+template <class T, bool REPEAT = false>
+DEVI void f32_load(f32x4 (&r)[T::kPer], const float* src, int end, int H, int head, int t0) {
+  constexpr int HD = T::kHd;
 #pragma unroll
   for (int i = 0; i < T::kPer; ++i) {
     const int x = threadIdx.x + i * T::kThreads, part = x % (4 * T::NR);
@@ -1431,9 +1436,8 @@ DEVI void f32_load(f32x4 (&r)[F32Tile<HD>::kPer], const float* src, int end, int
     if (t < end && part < HD / 4) r[i] = *reinterpret_cast<const f32x4*>(src + ((size_t)t * H + head) * HD + 4 * part);
   }
 }
-template <int HD>
-DEVI void f32_store(float (*dst)[F32Tile<HD>::kStride], const f32x4 (&r)[F32Tile<HD>::kPer]) {
-  using T = F32Tile<HD>;
+template <class T>
+DEVI void f32_store(float (*dst)[T::kStride], const f32x4 (&r)[T::kPer]) {
 #pragma unroll
   for (int i = 0; i < T::kPer; ++i) {
     const int x = threadIdx.x + i * T::kThreads;
@@ -1478,16 +1482,16 @@ DEVI f32x4 f32_product(const f32x4 (&p)[F32Tile<HD>::NR], const f32x4 (&o)[F32Ti
   return s;
 }
 // acc[b] += over the 16 partners from p0: partner's row times w[b] (partner 4 grp + r in w[b][r]), for QB owned blocks.
-template <int HD>
-DEVI void f32_gather(f32x4 (&acc)[F32Tile<HD>::QB][F32Tile<HD>::NR], const float (*rows)[F32Tile<HD>::kStride], int p0,
-                     const f32x4 (&w)[F32Tile<HD>::QB], int c16, int grp) {
+template <int HD, int QB>
+DEVI void f32_gather(f32x4 (&acc)[QB][F32Tile<HD>::NR], const float (*rows)[F32Tile<HD>::kStride], int p0,
+                     const f32x4 (&w)[QB], int c16, int grp) {
 #pragma unroll
   for (int c = 0; c < F32Tile<HD>::NR; ++c)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = rows[p0 + 4 * grp + r][16 * c + c16];
 #pragma unroll
-      for (int b = 0; b < F32Tile<HD>::QB; ++b) acc[b][c] = mfma16x4f(x, w[b][r], acc[b][c]);
+      for (int b = 0; b < QB; ++b) acc[b][c] = mfma16x4f(x, w[b][r], acc[b][c]);
     }
 }
 
@@ -1496,10 +1500,10 @@ DEVI void f32_gather(f32x4 (&acc)[F32Tile<HD>::QB][F32Tile<HD>::NR], const float
 // 64 / 340 / 3,000 keys): 1.8 / 2.3 / 3.6e-7, in one chain 2.1 / 3.8 / 10.4e-7, in the per-thread kernels' four key
 // splits 1.9 / 2.6 / 5.9e-7.  It takes 8-32 registers more, for which the unmasked forward is held to four waves per
 // SIMD: 8 heads of 32 over 64 small molecules 127 us in one chain, 129 held, 133 at the three waves it would take.
-template <int HD>
-DEVI void f32_add_stage(f32x4 (&acc)[F32Tile<HD>::QB][F32Tile<HD>::NR], const float (*rows)[F32Tile<HD>::kStride],
-                        const f32x4 (&w)[kF32Stage / 16][F32Tile<HD>::QB], int c16, int grp) {
-  constexpr int NR = F32Tile<HD>::NR, QB = F32Tile<HD>::QB;
+template <int HD, int QB>
+DEVI void f32_add_stage(f32x4 (&acc)[QB][F32Tile<HD>::NR], const float (*rows)[F32Tile<HD>::kStride],
+                        const f32x4 (&w)[kF32Stage / 16][QB], int c16, int grp) {
+  constexpr int NR = F32Tile<HD>::NR;
 #pragma unroll
   for (int kb = 0; kb < kF32Stage / 16; kb += 2) {
     f32x4 part[QB][NR];
@@ -1525,18 +1529,18 @@ DEVI void f32_add_stage(f32x4 (&acc)[F32Tile<HD>::QB][F32Tile<HD>::NR], const fl
 // walk and 149 without any check; dQ 127, 123 and 119).  They are held to the four waves for it; neither spills.  The
 // forward has no such walk: an infinite or NaN row of V reaches every query of its segment, as it does in the softmax of
 // a mask of -inf, whose zeros multiply V.
-template <int HD>
-DEVI void f32_gather_admissible(f32x4 (&acc)[F32Tile<HD>::QB][F32Tile<HD>::NR],
-                                const float (*rows)[F32Tile<HD>::kStride], int p0, const f32x4 (&w)[F32Tile<HD>::QB],
-                                int c16, int grp, const int2* nodes, int t0, int end, const int (&tok)[F32Tile<HD>::QB],
-                                const int2 (&node)[F32Tile<HD>::QB]) {
+template <int HD, int QB>
+DEVI void f32_gather_admissible(f32x4 (&acc)[QB][F32Tile<HD>::NR],
+                                const float (*rows)[F32Tile<HD>::kStride], int p0, const f32x4 (&w)[QB],
+                                int c16, int grp, const int2* nodes, int t0, int end, const int (&tok)[QB],
+                                const int2 (&node)[QB]) {
 #pragma unroll 1
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int p = p0 + 4 * j + r;
 #pragma unroll
-      for (int b = 0; b < F32Tile<HD>::QB; ++b) {
+      for (int b = 0; b < QB; ++b) {
         const float x = __shfl(w[b][r], 16 * j + c16);
         if (!admissible_f32<true>(t0 + p, end, tok[b], nodes[p], node[b])) continue;
 #pragma unroll
@@ -1558,9 +1562,8 @@ DEVI bool nonfinite(const f32x4 (&r)[N]) {
 }
 
 // The block's work item, the wave's column blocks and this lane's owned tokens (clamped into the group).
-template <int HD>
+template <int HD, int QB>
 struct F32Own {
-  static constexpr int QB = F32Tile<HD>::QB;
   int plo, phi, tok[QB];
   bool live, valid[QB];   // live: the wave owns a token (wave-uniform)
   DEVI F32Own(const int4& g, int wave, int c16) {
@@ -1593,10 +1596,12 @@ DEVI void f32_stages(int lo, int hi, bool live, Load load, Store store, Use use)
   }
 }
 
-template <bool MASKED, int HD, bool DROP, bool BIAS = false>
-__global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
-    MASKED ? 1 : 4))) void attn_fwd_f32_kernel(const AttnF32Args a) {
-  using T = F32Tile<HD>;
+// With a bias, head dims 24 and 32 spill a dozen registers at four waves a SIMD; at three they take 2 to 5 % less time
+// (600 segments of 60 tokens, 8 heads of 24 dims: 67 against 71 us).
+template <bool MASKED, int HD, bool DROP, bool BIAS = false, int TOK = kGroupTok>
+__global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_per_eu(
+    MASKED ? 1 : BIAS && (HD == 24 || HD == 32) ? 3 : 4))) void attn_fwd_f32_kernel(const AttnF32Args a) {
+  using T = F32Tile<HD, TOK>;
   constexpr int NR = T::NR, QB = T::QB, KB = kF32Stage / 16;
   __shared__ __align__(16) typename T::Rows sK[2], sV[2];
   __shared__ int2 sN[2][MASKED ? kF32Stage : 1];
@@ -1605,7 +1610,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   if (item >= *a.count) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, grp = lane >> 4;
-  const F32Own<HD> own(a.plan[item], wave, c16);
+  const F32Own<HD, QB> own(a.plan[item], wave, c16);
   const int phi = own.phi;
   f32x4 q[QB][NR], acc[QB][NR];
   int2 node[QB];
@@ -1629,14 +1634,14 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   f32_stages(
       own.plo, phi, own.live,
       [&](int t0) {
-        f32_load<HD>(rK, a.k, phi, H, head, t0);
-        f32_load<HD>(rV, a.v, phi, H, head, t0);
+        f32_load<T>(rK, a.k, phi, H, head, t0);
+        f32_load<T>(rV, a.v, phi, H, head, t0);
         if (MASKED && tid < kF32Stage) rN = t0 + tid < phi ? a.nodes[t0 + tid] : make_int2(-1, -1);
         if (DROP && tid < kF32Stage) rKey = drop_col(a.drop, t0 + tid);
       },
       [&](int buf) {
-        f32_store<HD>(sK[buf], rK);
-        f32_store<HD>(sV[buf], rV);
+        f32_store<T>(sK[buf], rK);
+        f32_store<T>(sV[buf], rV);
         if (MASKED && tid < kF32Stage) sN[buf][tid] = rN;
         if (DROP && tid < kF32Stage) sKey[buf][tid] = rKey;
       },
@@ -1918,10 +1923,10 @@ __global__ __launch_bounds__(256) void attn_dkdv_few_kernel(const AttnFewArgs a)
 }
 
 // dQ = scale * sum_j P_ij (dP_ij - D_i) k_j, P recomputed from the saved LSE.
-template <bool MASKED, int HD, bool DROP, bool BIAS = false>
-__global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
+template <bool MASKED, int HD, bool DROP, bool BIAS = false, int TOK = kGroupTok>
+__global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 4 : 1))) void attn_dq_f32_kernel(const AttnF32Args a) {
-  using T = F32Tile<HD>;
+  using T = F32Tile<HD, TOK>;
   constexpr int NR = T::NR, QB = T::QB, KB = kF32Stage / 16;
   __shared__ __align__(16) typename T::Rows sK[2], sV[2];
   __shared__ int2 sN[2][MASKED ? kF32Stage : 1];
@@ -1930,7 +1935,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   if (item >= *a.count) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, grp = lane >> 4;
-  const F32Own<HD> own(a.plan[item], wave, c16);
+  const F32Own<HD, QB> own(a.plan[item], wave, c16);
   const int phi = own.phi;
   f32x4 q[QB][NR], g[QB][NR], acc[QB][NR];
   int2 node[QB];
@@ -1961,14 +1966,14 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
     f32_stages(
         own.plo, phi, own.live,
         [&](int t0) {
-          f32_load<HD>(rK, a.k, phi, H, head, t0);
-          f32_load<HD>(rV, a.v, phi, H, head, t0);
+          f32_load<T>(rK, a.k, phi, H, head, t0);
+          f32_load<T>(rV, a.v, phi, H, head, t0);
           if (MASKED && tid < kF32Stage) rN = t0 + tid < phi ? a.nodes[t0 + tid] : make_int2(-1, -1);
           if (DROP && tid < kF32Stage) rKey = drop_col(a.drop, t0 + tid);
         },
         [&](int buf) {
-          f32_store<HD>(sK[buf], rK);
-          f32_store<HD>(sV[buf], rV);
+          f32_store<T>(sK[buf], rK);
+          f32_store<T>(sV[buf], rV);
           if (MASKED) odd |= nonfinite(rK);
           if (MASKED && tid < kF32Stage) sN[buf][tid] = rN;
           if (DROP && tid < kF32Stage) sKey[buf][tid] = rKey;
@@ -2046,10 +2051,10 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
 }
 
 // dV = sum_i P_ij dO_i, dK = scale * sum_i P_ij (dP_ij - D_i) q_i; the partners are queries with their (LSE2, D).
-template <bool MASKED, int HD, bool DROP, bool BIAS = false>
-__global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_per_eu(
+template <bool MASKED, int HD, bool DROP, bool BIAS = false, int TOK = kGroupTok>
+__global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 4 : 1))) void attn_dkdv_f32_kernel(const AttnF32Args a) {
-  using T = F32Tile<HD>;
+  using T = F32Tile<HD, TOK>;
   constexpr int NR = T::NR, QB = T::QB, KB = kF32Stage / 16;
   __shared__ __align__(16) typename T::Rows sQ[2], sG[2];
   __shared__ __align__(16) float sL[2][kF32Stage], sD[2][kF32Stage];
@@ -2059,7 +2064,7 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
   if (item >= *a.count) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, grp = lane >> 4;
-  const F32Own<HD> own(a.plan[item], wave, c16);
+  const F32Own<HD, QB> own(a.plan[item], wave, c16);
   const int phi = own.phi;
   f32x4 kx[QB][NR], vx[QB][NR], dk[QB][NR], dv[QB][NR];
   int2 node[QB];
@@ -2086,8 +2091,8 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
         [&](int t0) {
           // past the queries' end, without a mask to select by: the last one again.  An infinity of a key times a zero
           // row would be a NaN, where this row's score minus its infinite LSE2 is one only if the query's own is
-          f32_load<HD, !MASKED>(rQ, a.q, phi, H, head, t0);
-          f32_load<HD>(rG, a.dout, phi, H, head, t0);
+          f32_load<T, !MASKED>(rQ, a.q, phi, H, head, t0);
+          f32_load<T>(rG, a.dout, phi, H, head, t0);
           if (tid < kF32Stage) {
             const bool in = t0 + tid < phi;
             rR = in ? a.rows[(size_t)head * a.tq_pad + t0 + tid] : make_float2(INFINITY, 0.f);
@@ -2096,8 +2101,8 @@ __global__ __launch_bounds__(F32Tile<HD>::kThreads) __attribute__((amdgpu_waves_
           }
         },
         [&](int buf) {
-          f32_store<HD>(sQ[buf], rQ);
-          f32_store<HD>(sG[buf], rG);
+          f32_store<T>(sQ[buf], rQ);
+          f32_store<T>(sG[buf], rG);
           if (MASKED) odd |= nonfinite(rQ) || nonfinite(rG);
           if (tid < kF32Stage) {
             sL[buf][tid] = rR.x;
@@ -2730,8 +2735,14 @@ AttnFewArgs few_args(const void* q, const void* k, const void* v, const int* cu_
 
 // ---- with a relative position bias (the calls of esa_rel_attn.hip)
 #define ESA_F32_REL_K(KERNEL, HD, D, grid, lds, st, a)                                                             \
-  hipLaunchKernelGGL((KERNEL<false, HD, D, true>), grid, dim3(F32Tile<HD>::kThreads), lds(F32Tile<HD>::kThreads / 64), \
-                     st, a)
+  do {                                                                                                             \
+    if (a.group_tok == kFewTok)                                                                                    \
+      hipLaunchKernelGGL((KERNEL<false, HD, D, true, kFewTok>), grid, dim3(f32_threads(HD, kFewTok)),              \
+                         lds(f32_threads(HD, kFewTok) / 64), st, a);                                               \
+    else                                                                                                           \
+      hipLaunchKernelGGL((KERNEL<false, HD, D, true>), grid, dim3(F32Tile<HD>::kThreads),                          \
+                         lds(F32Tile<HD>::kThreads / 64), st, a);                                                  \
+  } while (0)
 #define ESA_F32_REL_HD(KERNEL, D, hd, grid, lds, st, a)                 \
   do {                                                                  \
     if (hd == 16) ESA_F32_REL_K(KERNEL, 16, D, grid, lds, st, a);       \
@@ -2753,10 +2764,11 @@ AttnF32Args f32_rel_args(const DenseAttnCall& c, const RelPass& r) {
   a.drop = c.drop;
   a.rel = r.bias;
   a.plan = r.plan_q; a.count = r.count_q; a.shift = r.shift_q;
+  a.group_tok = r.group_tok;
   return a;
 }
-dim3 f32_rel_grid(int total, const DenseAttnCall& c) {
-  return dim3((unsigned)(groups_of(total) + std::min(c.nseg, total)) * (unsigned)c.heads);
+dim3 f32_rel_grid(int total, const DenseAttnCall& c, int tok) {
+  return dim3((unsigned)((total + tok - 1) / tok + std::min(c.nseg, total)) * (unsigned)c.heads);
 }
 
 // Scratch of esa_varlen_attn_fwd_noalloc: a file-scope device array, one
@@ -2800,7 +2812,7 @@ int f32_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipS
   a.o = static_cast<float*>(c.out); a.lse_out = c.lse;
   auto lds = [&](int) { return r.bias.stride * sizeof(float); };
   ESA_TIMED(esa_profile::kAttnFwd, st,
-            ESA_F32_REL_LAUNCH(attn_fwd_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c), lds, st, a));
+            ESA_F32_REL_LAUNCH(attn_fwd_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c, r.group_tok), lds, st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }
@@ -2823,12 +2835,12 @@ int f32_rel_bwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipS
   auto sums = [&](int waves) { return rel_dq_floats(r.bias.stride, waves) * sizeof(float); };
   if (c.total_q > 0)
     ESA_TIMED(esa_profile::kAttnBwdDq, st,
-              ESA_F32_REL_LAUNCH(attn_dq_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c), sums, st, a));
+              ESA_F32_REL_LAUNCH(attn_dq_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c, r.group_tok), sums, st, a));
   ESA_LAUNCH_CHECK();
   a.plan = r.plan_k; a.count = r.count_k; a.shift = r.shift_k;
   if (c.total_k > 0)
     ESA_TIMED(esa_profile::kAttnBwdDkdv, st,
-              ESA_F32_REL_LAUNCH(attn_dkdv_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_k, c), line, st, a));
+              ESA_F32_REL_LAUNCH(attn_dkdv_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_k, c, r.group_tok), line, st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }

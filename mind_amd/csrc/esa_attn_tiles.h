@@ -12,6 +12,7 @@ constexpr int kTile = 32;
 constexpr int kHd = 16;
 constexpr int kWaves = 4;
 constexpr int kGroupTok = kWaves * kTile;   // 128 tokens per block
+constexpr int kFewTok = 64;                 // and of the fp32 kernels with a bias where the blocks are few
 constexpr int kRowStride = 24;              // bf16 per row of a [32 tokens][16] LDS tile (48 B)
 constexpr int kTrStride = 40;               // bf16 per row of a [rows][32 tokens] LDS tile (80 B)
 constexpr float kStaticBound = 60.f;

@@ -26,6 +26,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;    // values a block takes
 constexpr int kTable = 160;     // tensors a launch: 3.9 KB of kernel arguments
+// Up to so many sums the clipping's blocks join them by themselves, a launch less.  Norm and clipping of 4, 200, 480
+// and 1,000 chunks took 5.1, 8.1, 10.6 and 17.6 us, with the join's launch 6.6, 9.4, 11.7 and 17.5 (in a graph).
+constexpr int kOwnJoin = 512;
 constexpr int kInF32 = 1, kOutF32 = 2;
 
 struct Table {
@@ -176,10 +179,29 @@ DEVI void clip_chunk(const Chunk& c, float factor) {
       [&](int i, float x) { o[i] = (TO)(x * factor); });
 }
 
+// JOINS: no join launch went before; every block joins the `parts` sums by itself, and the first notes the norm.
+template <bool JOINS, bool MAX>
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Chunk* __restrict__ chunks, float max_norm,
-                                                             const float* __restrict__ norm) {
+                                                             float* __restrict__ norm, const double* __restrict__ part, int parts) {
+  __shared__ double s[kThreads / 64];
+  __shared__ float joined;
   const Chunk c = chunks[blockIdx.x];
-  const float f = max_norm / (*norm + 1e-6f), factor = f > 1.f ? 1.f : f;   // a NaN stays one
+  float n;
+  if (JOINS) {
+    Norm<MAX> sum;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < parts; i += kThreads) sum.join(part[i]);
+    const double v = block_join(sum, s);
+    if (threadIdx.x == 0) {
+      joined = (float)(MAX ? v : sqrt(v));
+      if (blockIdx.x == 0) *norm = joined;
+    }
+    __syncthreads();
+    n = joined;
+  } else {
+    n = *norm;
+  }
+  const float f = max_norm / (n + 1e-6f), factor = f > 1.f ? 1.f : f;   // a NaN stays one
   if (c.kind & kInF32) clip_chunk<float, float>(c, factor);
   else if (c.kind & kOutF32) clip_chunk<bf16, float>(c, factor);
   else clip_chunk<bf16, bf16>(c, factor);
@@ -243,6 +265,7 @@ int norm_launches(int n, const void* const* in, void* const* out, const long lon
     }
   }
   if (const int rc = flush()) return rc;
+  if (out && done > 0 && done <= kOwnJoin) return ESA_OK;   // the clipping joins
   ESA_TIMED(esa_profile::kGradNorm, st,
             hipLaunchKernelGGL((grad_norm_join_kernel<MAX>), dim3(1), dim3(1024), 0, st, part, done, norm));
   ESA_LAUNCH_CHECK();
@@ -304,8 +327,10 @@ int esa_grad_clip(int n, const void* const* in, void* const* out, const long lon
   auto go = infinity ? norm_launches<true> : norm_launches<false>;
   if ((rc = go(n, in, out, counts, in_dtypes, out_dtypes, norm, static_cast<double*>(workspace), chunks, st))) return rc;
   if (!total) return ESA_OK;
+  const double* part = static_cast<const double*>(workspace);
+  auto kernel = total > kOwnJoin ? grad_clip_kernel<false, false> : infinity ? grad_clip_kernel<true, true> : grad_clip_kernel<true, false>;
   ESA_TIMED(esa_profile::kGradClip, st,
-            hipLaunchKernelGGL(grad_clip_kernel, dim3(total), dim3(kThreads), 0, st, chunks, max_norm, norm));
+            hipLaunchKernelGGL(kernel, dim3(total), dim3(kThreads), 0, st, chunks, max_norm, norm, part, (int)total));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }

@@ -42,9 +42,21 @@ __global__ __launch_bounds__(kReduceCols* kReduceRows) void rel_reduce_kernel(co
 
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 int tiles32(int x) { return (x + kTile - 1) / kTile; }
-// At most ceil(T / 128) + (non-empty segments) groups, one more where they begin at even tokens.
-size_t groups_most(int total, int batch) {
-  return (size_t)(total + kGroupTok - 1) / kGroupTok + (size_t)std::min(batch, total) + 1;
+// At most ceil(T / tok) + (non-empty segments) groups, one more where they begin at even tokens.
+size_t groups_most(int total, int batch, int tok = kGroupTok) {
+  return (size_t)(total + tok - 1) / tok + (size_t)std::min(batch, total) + 1;
+}
+
+// Tokens of a group of the fp32 kernels.  A block walks its segment's partners alone, so with few blocks the walk of the
+// longest segment is the time, and groups of 64, half the work for a block, take less of it; with many blocks a group of
+// 128 feeds twice the products from each staged row.  A forward, and a step with its gradients, by blocks of 128 (8 heads;
+// us with groups of 128 -> 64): head dim 16, 184 blocks 31, 105 -> 22, 72; 616: 49, 176 -> 41, 149; 1,872: 87, 328 -> 84,
+// 316; 2,992 (32 proteins): 455, 1725 -> 458, 1765.  Head dim 64: 184: 58, 234 -> 40, 154; 376: 77, 274 -> 59, 230; 568
+// (8 proteins): 264, 1072 -> 271, 1094; 1,872: 224, 1083 -> 244, 1066.
+int group_tokens(int batch, int total_q, int total_k, int heads, int head_dim, int dtype) {
+  if (dtype != ESA_F32) return kGroupTok;
+  const size_t few = head_dim == 64 ? 512 : 2048;
+  return groups_most(std::max(total_q, total_k), batch) * heads <= few ? kFewTok : kGroupTok;
 }
 
 // The bf16 forward of few queries (at most 32 a segment on average) over many keys (512 and more): with a block per
@@ -74,8 +86,9 @@ Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int 
   };
   const int stride = 2 * (reach + kRelPad) + 1;
   const int split = split_keys(batch, total_q, total_k, heads, dtype, backward);
-  const size_t gk = groups_most(total_k, batch);
-  const size_t gq = split ? split_most(batch, total_q, total_k, split) : groups_most(total_q, batch);
+  const int tok = group_tokens(batch, total_q, total_k, heads, head_dim, dtype);
+  const size_t gk = groups_most(total_k, batch, tok);
+  const size_t gq = split ? split_most(batch, total_q, total_k, split) : groups_most(total_q, batch, tok);
   w.counts = take(8);
   w.plan_q = take(gq * sizeof(int4));
   w.shift_q = take(gq * sizeof(int));
@@ -165,7 +178,7 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
   p.zero_k = static_cast<uint4*>(c.dk); p.zero_v = static_cast<uint4*>(c.dv);
   p.lse = backward ? nullptr : c.lse;
   p.backward = backward;
-  p.gtok_q = kGroupTok;
+  p.gtok_q = p.gtok_k = r.group_tok = group_tokens(c.nseg, c.total_q, c.total_k, c.heads, c.head_dim, dtype);
   p.key_pairs = backward && c.dropout && dtype == ESA_BF16;   // the bf16 dK/dV pass shares its hashes by key pairs
 }
 

@@ -62,12 +62,13 @@ DEVI int2 split_groups(int queries, int keys, int per) {
 // What a call's attention passes read besides its tensors.
 struct RelPass {
   RelBias bias;
-  int4* plan_q; int4* plan_k;       // groups of 128 tokens (seg_plan_block); plan_k backward only
+  int4* plan_q; int4* plan_k;       // groups of 128 or 64 tokens (seg_plan_block); plan_k backward only
   int* count_q; int* count_k;
   int* shift_q; int* shift_k;       // per group: d = key token - query token - shift
   float* knorm; int tk_tiles;       // bf16 forward: max |k| per (head, 32-key tile)
   float2* rows; int tq_pad;         // backward: row statistics [heads][tq_pad]
   RelSplit split;                   // bf16 forward of few queries
+  int group_tok;   // fp32: tokens of a group
 };
 
 // The preparation: plans, bias lines and the rows of tokens in no segment.
@@ -79,7 +80,7 @@ struct RelPrep {
   float* line; float* top; int2* ranges;
   uint4* zero_q; uint4* zero_k; uint4* zero_v; float* lse;          // out or dq; dk, dv; forward: lse
   bool backward, key_pairs;
-  int gtok_q;                                                       // tokens of a query group
+  int gtok_q, gtok_k;                                               // tokens of a group of queries, of keys
 };
 constexpr int kRelClearBlocks = 16;
 inline int rel_prep_blocks(const RelPrep& p) { return 1 + (p.backward ? 1 : 0) + p.heads + kRelClearBlocks; }
@@ -327,7 +328,7 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
   b -= 1;
   if (p.backward) {
     if (b == 0) {
-      seg_plan_block(p.cu_k, p.cu_q, p.nseg, kGroupTok, r.plan_k, r.count_k, tid, p.key_pairs, r.shift_k, shift_of);
+      seg_plan_block(p.cu_k, p.cu_q, p.nseg, p.gtok_k, r.plan_k, r.count_k, tid, p.key_pairs, r.shift_k, shift_of);
       return;
     }
     b -= 1;

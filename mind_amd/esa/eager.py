@@ -20,10 +20,15 @@ _transforms = torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._get_tracing_state
 
 
+def ordinary() -> bool:
+    """True in ordinary eager execution."""
+    return not (torch.compiler.is_compiling() or _dispatch_modes() or _function_modes() or _transforms() is not None
+                or forward_ad._current_level >= 0 or _tracing() is not None)
+
+
 def plain(*args) -> bool:
     """True in ordinary eager execution on ordinary tensors (arguments that are no tensors are not looked at)."""
-    if (torch.compiler.is_compiling() or _dispatch_modes() or _function_modes() or _transforms() is not None
-            or forward_ad._current_level >= 0 or _tracing() is not None):
+    if not ordinary():
         return False
     return all(type(a) in _PLAIN or not isinstance(a, torch.Tensor) for a in args)
 
@@ -51,5 +56,15 @@ class Unrecorded:
 def call(function, *args):
     """``function.apply(*args)`` of an autograd function; its forward alone where nothing records or traces it."""
     if not records(*args) and plain(*args):
+        return function.forward(Unrecorded(), *args)
+    return function.apply(*args)
+
+
+FITS, EXACT, GRAD = 1, 2, 4   # what the host module's checks say of a call (csrc/esa_tensors.cpp)
+
+
+def call_checked(flags: int, function, *args):
+    """``call`` where the host module has looked at the tensors."""
+    if flags & EXACT and not (flags & GRAD and torch.is_grad_enabled()) and ordinary():
         return function.forward(Unrecorded(), *args)
     return function.apply(*args)

@@ -78,7 +78,6 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
         return _norm(lists, infinity)
 
 
-@torch.no_grad()
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, error_if_nonfinite: bool = False) -> torch.Tensor:
     """The gradients times min(1, max_norm / (norm + 1e-6)), their norm (``grad_norm``) returned as a scalar on the
     device.
@@ -99,8 +98,20 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, err
         raise ValueError(f"out has {len(targets)} tensors for {len(grads)} gradients")
     if not grads:
         return torch.zeros(())
+    if not error_if_nonfinite and isinstance(grads[0], torch.Tensor) and grads[0].is_cuda:
+        done = _lib.tensors().clip(_lib.address("esa_grad_clip"), _lib.address("esa_grad_workspace_size"),
+                                   _lib.stream_of(grads[0]), grads, targets, infinity, max_norm)
+        if done is not None:
+            _lib.check(done[0], "esa_grad_clip")
+            return done[1]
+    return _clip_with_copies(grads, targets, max_norm, infinity, error_if_nonfinite)
+
+
+@torch.no_grad()
+def _clip_with_copies(grads, targets, max_norm: float, infinity: int, error_if_nonfinite: bool) -> torch.Tensor:
+    """``clip_gradients`` for lists of any layout, and what says why a call is refused."""
     src = _Lists(grads, _copy)
-    if out is None:
+    if targets is grads:
         dst = src
     else:
         dst = _Lists(targets, lambda o: torch.empty(o.shape, dtype=o.dtype, device=o.device))

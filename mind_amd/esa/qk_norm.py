@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .attention import HEAD_DIMS
-from .eager import call
+from .eager import FITS, call_checked
 from .layer_norm import f32_values
 from .linear import on_boundary
 
@@ -28,14 +28,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> t
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive (got {rotary_dim})")
     return float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x, or its copy where its rows are not 16-byte aligned runs."""
-    size = x.element_size()
-    if (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(q, k):
@@ -54,14 +46,10 @@ class _QkNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
         ctx.weight_dtypes = [None if w is None else w.dtype for w in (q_weight, k_weight)]
-        q, k = _rows(q), None if k is None else _rows(k)
         wq, wk = f32_values(q_weight), f32_values(k_weight)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        with _lib.on_device(q):
-            _lib.check(_lib.load().esa_qk_norm_fwd(
-                q.data_ptr(), _lib.ptr(k), _strides(q, k), *_common(q, k, wq, wk, positions, frequencies, interleaved, eps),
-                q_out.data_ptr(), _lib.ptr(k_out), _lib.stream_of(q)), "esa_qk_norm_fwd")
+        rc, q_out, k_out, q, k = _lib.tensors().qk_norm_forward(_lib.address("esa_qk_norm_fwd"), _lib.stream_of(q), q, k, wq, wk,
+                                                                positions, frequencies, eps, interleaved)
+        _lib.check(rc, "esa_qk_norm_fwd")
         ctx.save_for_backward(q, k, wq, wk, positions, frequencies)
         ctx.meta = (eps, interleaved)
         return (q_out, k_out) if k is not None else q_out
@@ -101,19 +89,8 @@ def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor | None = None) ->
         raise ValueError(f"{name} must have the tokens, head_dim and dtype of q (got {tuple(x.shape)}, {x.dtype})")
 
 
-def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, frequencies=None, eps=1e-6, interleaved=False):
-    """(q', k') of query rows q [T, Hq, hd] and key rows k [T, Hk, hd] (k None: q' alone); hd 16, 24, 32 or 64, float32
-    or bfloat16 with float32 arithmetic, rounded once.
-
-    y = x / sqrt(mean(x ** 2) + eps) * weight over each head's row; q_weight / k_weight: [hd] or None (ones).  With
-    ``positions`` (int32 or int64 [T], any values) and ``frequencies`` (float64 [r / 2], ``rotary_frequencies``; r a
-    multiple of 8 up to hd), the first r dimensions are rotated in pairs (i, i + r / 2), or (2i, 2i + 1) with
-    ``interleaved``, by positions * frequencies[i], worked out in 64 bits (an angle is off by at most 2^-51 of itself).
-
-    q and k may be views (of one projection's output, say): rows of hd consecutive elements on 16-byte boundaries are
-    read where they are, others from a copy.  The outputs are contiguous.  Gradients reach q, k and the weights (summed
-    in float32 in a fixed order), once: they cannot be differentiated again.
-    """
+def _check(q, k, q_weight, k_weight, positions, frequencies):
+    """Says what is wrong with a call that the host module found not to fit."""
     _check_rows("q", q)
     if k is not None:
         _check_rows("k", k, q)
@@ -136,10 +113,27 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, freq
         r = 2 * frequencies.numel()
         if r % 8 or not 8 <= r <= q.shape[2]:
             raise ValueError(f"frequencies must rotate a multiple of 8 dimensions up to head_dim {q.shape[2]} (got {r})")
+
+
+def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, frequencies=None, eps=1e-6, interleaved=False):
+    """(q', k') of query rows q [T, Hq, hd] and key rows k [T, Hk, hd] (k None: q' alone); hd 16, 24, 32 or 64, float32
+    or bfloat16 with float32 arithmetic, rounded once.
+
+    y = x / sqrt(mean(x ** 2) + eps) * weight over each head's row; q_weight / k_weight: [hd] or None (ones).  With
+    ``positions`` (int32 or int64 [T], any values) and ``frequencies`` (float64 [r / 2], ``rotary_frequencies``; r a
+    multiple of 8 up to hd), the first r dimensions are rotated in pairs (i, i + r / 2), or (2i, 2i + 1) with
+    ``interleaved``, by positions * frequencies[i], worked out in 64 bits (an angle is off by at most 2^-51 of itself).
+
+    q and k may be views (of one projection's output, say): rows of hd consecutive elements on 16-byte boundaries are
+    read where they are, others from a copy.  The outputs are contiguous.  Gradients reach q, k and the weights (summed
+    in float32 in a fixed order), once: they cannot be differentiated again.
+    """
+    flags = _lib.tensors().qk_norm_fits(q, k, q_weight, k_weight, positions, frequencies)
+    if not flags & FITS:
+        _check(q, k, q_weight, k_weight, positions, frequencies)
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative (got {eps})")
-    tensors = [t for t in (q, k, q_weight, k_weight, positions, frequencies) if t is not None]
-    _lib.require_gpu(*tensors)
-    _lib.require_one_device(*tensors)
-    return call(_QkNorm, q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))
+    if not flags & FITS:
+        _lib.require_on_one_gpu(q, k, q_weight, k_weight, positions, frequencies)
+    return call_checked(flags, _QkNorm, q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))

@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .attention import (_SEED_MASK, _check_dropout, _check_index, _check_tokens, _dtype_code, draw_dropout_seed)
-from .eager import call
+from .eager import FITS, call_checked
 from .linear import on_boundary
 
 MAX_REACH, MAX_BUCKETS = 768, 256
@@ -55,30 +55,19 @@ def bucket_starts(num_buckets: int, max_distance: int = 128, bidirectional: bool
     return tuple(starts)
 
 
-def _workspace(device, batch, tq, tk, heads, hd, dt, buckets, starts, backward):
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.load().esa_rel_attn_workspace_size(batch, tq, tk, heads, hd, dt, buckets, starts, len(starts),
-                                                       int(backward), ctypes.byref(n)), "esa_rel_attn_workspace_size")
-    return torch.empty(max(int(n.value), 256), dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=64)
+def _start_bytes(starts: tuple[int, ...]) -> bytes:
+    return bytes((ctypes.c_int * len(starts))(*starts))
 
 
 class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, cu_q, cu_k, q_start, starts, scale, dropout_p, seed):
-        (tq, heads, hd), tk, batch, dt = q.shape, k.shape[0], cu_q.numel() - 1, _dtype_code(q)
-        table = bias.contiguous()
-        out = torch.empty_like(q)
-        # what the rounding of out leaves, where a backward may need it: its row statistic is exact then
-        low = torch.empty_like(q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else None
-        lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device)
-        c_starts = (ctypes.c_int * len(starts))(*starts)
-        with _lib.on_device(q):
-            ws = _workspace(q.device, batch, tq, tk, heads, hd, dt, table.shape[0], c_starts, False)
-            _lib.check(_lib.load().esa_rel_attn_fwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), _TABLE[table.dtype], table.shape[0], c_starts,
-                len(starts), _lib.ptr(q_start), cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, heads, hd, dt, scale,
-                dropout_p, seed, out.data_ptr(), _lib.ptr(low), lse.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)),
-                "esa_rel_attn_fwd")
+        # kept for a backward: what the rounding of a bf16 out leaves, so that its row statistic has none
+        rc, out, low, lse, table = _lib.tensors().relative_forward(
+            _lib.address("esa_rel_attn_fwd"), _lib.address("esa_rel_attn_workspace_size"), _lib.stream_of(q), q, k, v, bias,
+            _start_bytes(starts), q_start, cu_q, cu_k, scale, dropout_p, seed, any(ctx.needs_input_grad))
+        _lib.check(rc, "esa_rel_attn_fwd")
         ctx.save_for_backward(q, k, v, table, out, low, lse, cu_q, cu_k, q_start)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
@@ -98,13 +87,37 @@ class _RelativeAttention(torch.autograd.Function):
         dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
         c_starts = (ctypes.c_int * len(starts))(*starts)
         with _lib.on_device(q):
-            ws = _workspace(q.device, batch, tq, tk, heads, hd, dt, table.shape[0], c_starts, True)
+            need = ctypes.c_size_t(0)
+            _lib.check(_lib.load().esa_rel_attn_workspace_size(batch, tq, tk, heads, hd, dt, table.shape[0], c_starts,
+                                                               len(starts), 1, ctypes.byref(need)),
+                       "esa_rel_attn_workspace_size")
+            ws = torch.empty(max(int(need.value), 256), dtype=torch.uint8, device=q.device)
             _lib.check(_lib.load().esa_rel_attn_bwd(
                 g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(low), lse.data_ptr(),
                 table.data_ptr(), _TABLE[table.dtype], table.shape[0], c_starts, len(starts), _lib.ptr(q_start), cu_q.data_ptr(),
                 cu_k.data_ptr(), batch, tq, tk, heads, hd, dt, scale, dropout_p, seed, dq.data_ptr(), dk.data_ptr(),
                 dv.data_ptr(), dtable.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)), "esa_rel_attn_bwd")
         return dq, dk, dv, dtable.to(table.dtype), None, None, None, None, None, None, None
+
+
+def _check(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start):
+    """Says what is wrong with a call that the host module found not to fit."""
+    _check_tokens("q", q)
+    heads, hd = q.shape[1], q.shape[2]
+    _check_tokens("k", k, heads, q.dtype, hd)
+    _check_tokens("v", v, heads, q.dtype, hd)
+    if k.shape[0] != v.shape[0]:
+        raise ValueError("k and v must have the same number of tokens")
+    if bias.dtype not in _TABLE:
+        raise TypeError(f"bias must be float32 or bfloat16 (got {bias.dtype})")
+    if bias.dim() != 2 or bias.shape[1] != heads:
+        raise ValueError(f"bias must be [num_buckets, heads = {heads}] (got {tuple(bias.shape)})")
+    _check_index("cu_seqlens_q", cu_seqlens_q)
+    batch = cu_seqlens_q.numel() - 1
+    if batch < 1:
+        raise ValueError("cu_seqlens_q must have at least two entries")
+    _check_index("cu_seqlens_k", cu_seqlens_k, batch + 1)
+    _check_index("q_start", q_start, batch)
 
 
 def relative_attention(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=None, max_seqlen_k=None, max_distance=128,
@@ -127,29 +140,15 @@ def relative_attention(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=N
     dropout_p = _check_dropout(dropout_p)
     if dropout_p > 0.0 and dropout_seed is None:
         dropout_seed = draw_dropout_seed()
-    _check_tokens("q", q)
-    heads, hd = q.shape[1], q.shape[2]
-    _check_tokens("k", k, heads, q.dtype, hd)
-    _check_tokens("v", v, heads, q.dtype, hd)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError("k and v must have the same number of tokens")
-    if bias.dtype not in _TABLE:
-        raise TypeError(f"bias must be float32 or bfloat16 (got {bias.dtype})")
-    if bias.dim() != 2 or bias.shape[1] != heads:
-        raise ValueError(f"bias must be [num_buckets, heads = {heads}] (got {tuple(bias.shape)})")
+    flags = _lib.tensors().relative_fits(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start)
+    if not flags & FITS:
+        _check(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start)
     starts = bucket_starts(bias.shape[0], max_distance, bool(bidirectional))
-    _check_index("cu_seqlens_q", cu_seqlens_q)
-    batch = cu_seqlens_q.numel() - 1
-    if batch < 1:
-        raise ValueError("cu_seqlens_q must have at least two entries")
-    _check_index("cu_seqlens_k", cu_seqlens_k, batch + 1)
-    _check_index("q_start", q_start, batch)
-    scale = 1.0 / math.sqrt(hd) if softmax_scale is None else float(softmax_scale)
+    scale = 1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"softmax_scale must be positive and finite (got {softmax_scale})")
-    tensors = [t for t in (q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start) if t is not None]
-    _lib.require_gpu(*tensors)
-    _lib.require_one_device(*tensors)
-    out, lse = call(_RelativeAttention, q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start, starts, scale, dropout_p,
-                    int(dropout_seed or 0) & _SEED_MASK)
+    if not flags & FITS:
+        _lib.require_on_one_gpu(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start)
+    out, lse = call_checked(flags, _RelativeAttention, q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start, starts, scale,
+                            dropout_p, int(dropout_seed or 0) & _SEED_MASK)
     return (out, lse) if return_lse else out

@@ -341,3 +341,27 @@ def test_refused_on_the_device(device):
     (grad,) = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.float().sum().backward()
+
+
+@pytest.mark.parametrize("hd", [16, 24, 32, 64])
+@pytest.mark.parametrize("dropout", [0.0, 0.2])
+def test_many_blocks_in_single_precision(device, hd, dropout):
+    """The fp32 kernels' groups of 128 tokens (more than 2,048 blocks of them; the other tests' few blocks take 64)."""
+    lens = [1 + (7 * i) % 19 for i in range(290)] + [0, 260, 129]
+    check(device, torch.float32, 7, hd, lens, dropout=dropout, seed=61, extra=3)
+
+
+@pytest.mark.parametrize("lens_q,lens_k", [([3, 0, 40], [900, 30, 0]), ([2, 1], [700, 1500])], ids=str)
+def test_split_forward_then_backward_with_rows_left_out(device, lens_q, lens_k):
+    """A segment without keys and a head whose table leaves everything out, after the forward that writes neither's
+    rounding residue: no gradient there, and none of the other rows is touched."""
+    q, k, v, g, b, cu_q, cu_k = case(device, torch.bfloat16, 2, 16, lens_q, lens_k, seed=63, extra=2)
+    b[:, 1] = -math.inf
+    junk = torch.full((1 << 22,), math.nan, device=device)   # what a fresh allocation finds
+    del junk
+    leaves = [x.requires_grad_(True) for x in (q, k, v, b)]
+    grads = torch.autograd.grad(relative_attention(*leaves, cu_q, cu_k), leaves, g)
+    ref = oracle(q, k, v, b.masked_fill(torch.isinf(b), -1e4), lens_q, lens_k, g=g)   # its head 1 is not compared
+    for got, want in zip(grads[:3], ref[2:5]):
+        assert not got[:, 1].any() and rel_err(got[:, 0], want[:, 0]) <= 6e-3
+    assert not grads[3][:, 1].any() and torch.isfinite(grads[3]).all()
