@@ -1656,17 +1656,14 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
         }
         const bool tail = k0 + kF32Stage > phi;
         if (BIAS) {
-          const int base = rel_base(a.rel, k0, first, shift);
-          bool far_hi;
-          const bool near = rel_near(a.rel, base, kF32Stage, 16 * QB, far_hi);
+          const int base = rel_within(a.rel, rel_base(a.rel, k0, first, shift), kF32Stage, 16 * QB);
           const float* line = sRel + base + 4 * grp - c16;
-          const float far = sRel[far_hi ? a.rel.stride - 1 : 0];
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int b = 0; b < QB; ++b)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[kb][b][r] = fmaf(s[kb][b][r], a.c, near ? line[16 * (kb - b) + r] : far);
+              for (int r = 0; r < 4; ++r) s[kb][b][r] = fmaf(s[kb][b][r], a.c, line[16 * (kb - b) + r]);
         }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -1983,7 +1980,7 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
           const int base = BIAS ? rel_base(a.rel, k0, first, shift) : 0;
           bool far_hi = false;
           const bool near = BIAS && rel_near(a.rel, base, kF32Stage, 16 * QB, far_hi);
-          const float far = BIAS ? sRel[far_hi ? a.rel.stride - 1 : 0] : 0.f;
+          const int within = BIAS ? rel_within(a.rel, base, kF32Stage, 16 * QB) : 0;
           float far_sum = 0.f;
           f32x4 kept[QB][KB];   // a near stage's dS
           auto block = [&](int kb) {
@@ -2000,8 +1997,8 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
               const int2 pn = MASKED ? sN[buf][key] : make_int2(0, 0);
 #pragma unroll
               for (int b = 0; b < QB; ++b) {
-                const int entry = base + key - 16 * b - c16;
-                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], near ? sRel[entry] : far) - rs[b].x
+                const int entry = within + key - 16 * b - c16;
+                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], sRel[entry]) - rs[b].x
                                                : a.c * s[b][r] - rs[b].x);
                 float dp = ds[b][r];
                 if (DROP) dp = drop_keep(a.drop, rk[b], sKey[buf][key], k0 + key) ? dp * a.drop.inv_keep : 0.f;
@@ -2112,10 +2109,7 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
           }
         },
         [&](int buf, int q0) {
-          const int base = BIAS ? rel_base(a.rel, first, q0, shift) : 0;
-          bool far_hi = false;
-          const bool near = BIAS && rel_near(a.rel, base, 16 * QB, kF32Stage, far_hi);
-          const float far = BIAS ? sRel[far_hi ? a.rel.stride - 1 : 0] : 0.f;
+          const int base = BIAS ? rel_within(a.rel, rel_base(a.rel, first, q0, shift), 16 * QB, kF32Stage) : 0;
           auto block = [&](int kb) {
             f32x4 x[NR], s[QB], ds[QB];
             f32_rows<HD>(x, sQ[buf], 16 * kb, c16, grp);
@@ -2132,7 +2126,7 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
 #pragma unroll
               for (int b = 0; b < QB; ++b) {
                 // a query past the range has LSE2 = inf
-                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], near ? sRel[base + 16 * b + c16 - qi] : far) - lse2[r]
+                const float p = fast_exp2(BIAS ? fmaf(a.c, s[b][r], sRel[base + 16 * b + c16 - qi]) - lse2[r]
                                                : a.c * s[b][r] - lse2[r]);
                 const bool in = !MASKED || admissible_f32<true>(q0 + qi, phi, own.tok[b], pn, node[b]);
                 const bool keep = !DROP || drop_keep(a.drop, sKey[buf][qi], ck[b], own.tok[b]);

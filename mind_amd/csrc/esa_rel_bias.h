@@ -110,6 +110,10 @@ DEVI bool rel_near(const RelBias& r, int base, int nk, int nq, bool& far_hi) {
   return !far_hi && base + nk - 1 > kRelPad;
 }
 
+// The base moved to where the same nk by nq tile's entries lie in the line: a tile beyond its ends reads their one value
+// from its pads (nk + nq - 2 entries lie within 96).  A tile then needs no case of its own where only scores are wanted.
+DEVI int rel_within(const RelBias& r, int base, int nk, int nq) { return min(max(base, nq - 1), r.stride - nk); }
+
 constexpr int kRelMaxStride = 2 * (kRelMaxReach + kRelPad) + 1;
 // All of a thread's loads first: one wait for them in a block's start, not one an entry.
 template <int THREADS>
