@@ -374,22 +374,23 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
   // rows of tokens in no segment: zeros, and an lse of -inf
   auto clear = [&](uint4* rows, const int* cu, int total) {
     if (!rows) return;
+    const size_t first = (size_t)min(max(cu[0], 0), total) * p.row16;
     const size_t from = (size_t)min(max(cu[p.nseg], 0), total) * p.row16, to = (size_t)total * p.row16;
+    for (size_t i = (size_t)b * 256 + tid; i < first; i += (size_t)kRelClearBlocks * 256) rows[i] = make_uint4(0, 0, 0, 0);
     for (size_t i = from + (size_t)b * 256 + tid; i < to; i += (size_t)kRelClearBlocks * 256)
       rows[i] = make_uint4(0, 0, 0, 0);
   };
   clear(p.zero_q, p.cu_q, p.total_q);
   clear(p.zero_k, p.cu_k, p.total_k);
   clear(p.zero_v, p.cu_k, p.total_k);
-  if (r.split.keys)
-    for (int t = min(max(p.cu_q[p.nseg], 0), p.total_q) + b * 256 + tid; t < p.total_q; t += kRelClearBlocks * 256)
-      r.split.where[t] = make_int4(0, 0, 0, 0);
-  if (p.lse) {
-    const int from = min(max(p.cu_q[p.nseg], 0), p.total_q);
-    for (int h = 0; h < p.heads; ++h)
-      for (int t = from + b * 256 + tid; t < p.total_q; t += kRelClearBlocks * 256)
-        p.lse[(size_t)h * p.total_q + t] = -INFINITY;
-  }
+  const int first = min(max(p.cu_q[0], 0), p.total_q), from = min(max(p.cu_q[p.nseg], 0), p.total_q);
+  auto each = [&](auto use) {
+    for (int t = b * 256 + tid; t < first; t += kRelClearBlocks * 256) use(t);
+    for (int t = from + b * 256 + tid; t < p.total_q; t += kRelClearBlocks * 256) use(t);
+  };
+  if (r.split.keys) each([&](int t) { r.split.where[t] = make_int4(0, 0, 0, 0); });
+  if (p.lse)
+    for (int h = 0; h < p.heads; ++h) each([&](int t) { p.lse[(size_t)h * p.total_q + t] = -INFINITY; });
 }
 
 }  // namespace

@@ -232,7 +232,7 @@ struct Args {
     if (!THPVariable_CheckTypeExact(Py_TYPE(o))) flags &= ~kExact;
     if (t.requires_grad()) flags |= kGrad;
     if (!first) first = &t;
-    if (t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != first->get_device()) flags &= ~kFits;
+    if (t.layout() != at::kStrided || t.is_neg() || !t.is_cuda() || t.get_device() != first->get_device()) flags &= ~kFits;
     return &t;
   }
   void want(bool ok) { flags = ok ? flags : flags & ~kFits; }

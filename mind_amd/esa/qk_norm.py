@@ -136,4 +136,6 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, freq
         raise ValueError(f"eps must be finite and not negative (got {eps})")
     if not flags & FITS:
         _lib.require_on_one_gpu(q, k, q_weight, k_weight, positions, frequencies)
+        q, k, q_weight, k_weight, frequencies = (None if t is None else t.resolve_neg()
+                                                 for t in (q, k, q_weight, k_weight, frequencies))
     return call_checked(flags, _QkNorm, q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))

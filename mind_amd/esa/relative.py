@@ -149,6 +149,7 @@ def relative_attention(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=N
         raise ValueError(f"softmax_scale must be positive and finite (got {softmax_scale})")
     if not flags & FITS:
         _lib.require_on_one_gpu(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start)
+        q, k, v, bias = (t.resolve_neg() for t in (q, k, v, bias))
     out, lse = call_checked(flags, _RelativeAttention, q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start, starts, scale,
                             dropout_p, int(dropout_seed or 0) & _SEED_MASK)
     return (out, lse) if return_lse else out

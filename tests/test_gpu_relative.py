@@ -365,3 +365,37 @@ def test_split_forward_then_backward_with_rows_left_out(device, lens_q, lens_k):
     for got, want in zip(grads[:3], ref[2:5]):
         assert not got[:, 1].any() and rel_err(got[:, 0], want[:, 0]) <= 6e-3
     assert not grads[3][:, 1].any() and torch.isfinite(grads[3]).all()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 32), (torch.float32, 16)])
+@pytest.mark.parametrize("lens_q,lens_k", [([40, 90], [40, 90]), ([2, 1], [900, 700])], ids=["whole", "few"])
+def test_segments_that_begin_behind_the_first_token(device, dtype, hd, lens_q, lens_k):
+    """Tokens before the first segment belong to none, as those behind the last."""
+    q, k, v, g, b, cu_q, cu_k = case(device, dtype, 2, hd, lens_q, lens_k, seed=71)
+    around = lambda x, n, v=math.nan: torch.cat([x.new_full((n, *x.shape[1:]), v), x, x.new_full((2, *x.shape[1:]), v)])
+    junk = [torch.full((1 << 20,), math.nan, device=device) for _ in range(4)]   # what fresh allocations find
+    del junk
+    plain = [x.requires_grad_(True) for x in (q, k, v, b)]
+    out, lse = relative_attention(*plain, cu_q, cu_k, return_lse=True)
+    grads = torch.autograd.grad(out, plain, g)
+    moved = [around(q.detach(), 5), around(k.detach(), 3), around(v.detach(), 3), b.detach().clone()]
+    moved = [x.requires_grad_(True) for x in moved]
+    out2, lse2 = relative_attention(*moved, cu_q + 5, cu_k + 3, return_lse=True)
+    grads2 = torch.autograd.grad(out2, moved, around(g, 5, 1.0))
+    assert torch.equal(out2[5:-2], out) and not out2[:5].any() and not out2[-2:].any()
+    assert torch.equal(lse2[:, 5:-2], lse) and bool(torch.isneginf(lse2[:, :5]).all())
+    for x, y, n in zip(grads2[:3], grads[:3], (5, 3, 3)):
+        assert torch.equal(x[n:-2], y) and not x[:n].any() and not x[-2:].any()
+    assert torch.equal(grads2[3], grads[3])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_keys_and_negative_views(device, dtype):
+    q, k, v, g, b, cu_q, _ = case(device, dtype, 2, 32, [3, 70], seed=73)
+    leaves = [x.requires_grad_(True) for x in (q, k[:0].clone(), v[:0].clone(), b)]
+    out, lse = relative_attention(*leaves, cu_q, torch.zeros_like(cu_q), return_lse=True)
+    grads = torch.autograd.grad(out, leaves, g)
+    assert not out.any() and bool(torch.isneginf(lse).all()) and not any(x.any() for x in grads)
+    with torch.no_grad():
+        want = relative_attention(-q, k, v, b, cu_q, cu_q)
+        assert torch.equal(relative_attention(torch._neg_view(q), k, v, b, cu_q, cu_q), want)
