@@ -201,3 +201,41 @@ def test_refused(device):
                                 ((g, 1.0), {"out": [torch.zeros(5, device=device, dtype=torch.bfloat16)]}, TypeError)):
         with pytest.raises(error):
             clip_gradients(*args, **kwargs)
+
+
+@pytest.mark.parametrize("chunks", [1, 511, 512, 513, 1500])
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_joined_by_the_clipping_or_before_it(device, chunks, norm_type):
+    """Up to 512 chunks of 8,192 values the clipping's blocks join the norm themselves; the norm alone never does."""
+    flat = torch.randn(chunks * 8192 - 5, device=device, generator=torch.Generator(device).manual_seed(chunks))
+    grads = list(flat.split([1, 8191, flat.numel() - 8192])) if chunks > 1 else [flat]
+    want = float(flat.double().abs().max()) if norm_type == math.inf else float(flat.double().norm())
+    before = flat.double()
+    alone = grad_norm(grads, norm_type)
+    norm = clip_gradients(grads, want / 4, norm_type)
+    assert torch.equal(norm, alone) and abs(float(norm) - want) <= 1e-7 * want
+    close(flat, before * min(1.0, want / 4 / (float(norm) + 1e-6)), torch.float32)
+    flat[-1] = math.nan
+    assert math.isnan(float(clip_gradients(grads, 1.0, norm_type))) and bool(torch.isnan(flat).all())
+
+
+def test_two_calls_at_once(device):
+    a, b = (make(device, SIZES, (torch.float32, torch.bfloat16), seed) for seed in (5, 6))
+    want = [[clip_gradients(x, 0.5, out=[torch.empty_like(t) for t in x])] for x in (a, b)]
+    outs = [[torch.empty_like(t) for t in x] for x in (a, b)]
+    ref = [[torch.empty_like(t) for t in x] for x in (a, b)]
+    for x, o in zip((a, b), ref):
+        clip_gradients(x, 0.5, out=o)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    norms = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                norms[i].append(clip_gradients((a, b)[i], 0.5, out=outs[i]))
+    for s in sides:
+        torch.cuda.current_stream().wait_stream(s)
+    for i in (0, 1):
+        assert all(torch.equal(n, want[i][0]) for n in norms[i])
+        assert all(torch.equal(x, y) for x, y in zip(outs[i], ref[i]))

@@ -399,3 +399,64 @@ def test_no_keys_and_negative_views(device, dtype):
     with torch.no_grad():
         want = relative_attention(-q, k, v, b, cu_q, cu_q)
         assert torch.equal(relative_attention(torch._neg_view(q), k, v, b, cu_q, cu_q), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_graphs_in_turn_with_few_queries(device, dtype):
+    """Two captured forwards over keys cut into groups (bf16; one launch in fp32), replayed in turn with new inputs and
+    lengths between eager calls."""
+    made = [case(device, dtype, 3, 32, lens_q, lens_k, seed=81 + i) for i, (lens_q, lens_k) in
+            enumerate((([3, 1], [900, 1100]), ([2, 2, 5], [2000, 40, 700])))]
+    graphs, held = [], []
+    for q, k, v, _, b, cu_q, cu_k in made:
+        with torch.no_grad():
+            relative_attention(q, k, v, b, cu_q, cu_k)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held.append(relative_attention(q, k, v, b, cu_q, cu_k, return_lse=True))
+            graphs.append(graph)
+    for seed in (1, 2, 3):
+        for q, k, v, _, b, cu_q, cu_k in made:
+            for x in (q, k, v, b):
+                x.copy_(seeded_normal(tuple(x.shape), 100 * seed + x.shape[0], torch.float32))
+            cu_q[1] += 1 if seed == 2 else 0   # the lengths are read on the device
+        for graph in graphs:
+            graph.replay()
+        for (q, k, v, _, b, cu_q, cu_k), (out, lse) in zip(made, held):
+            with torch.no_grad():
+                want = relative_attention(q, k, v, b, cu_q, cu_k, return_lse=True)
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 64), (torch.float32, 24)])
+def test_two_calls_at_once(device, dtype, hd):
+    made = [case(device, dtype, 4, hd, lens, seed=91 + i) for i, lens in enumerate(([300, 77, 512], [64, 700]))]
+
+    def step(i):
+        q, k, v, g, b, cu, _ = made[i]
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v, b)]
+        out = relative_attention(*leaves, cu, cu)
+        return (out, *torch.autograd.grad(out, leaves, g))
+    want = [step(0), step(1)]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in sides:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    for s in sides:
+        torch.cuda.current_stream().wait_stream(s)
+    for i in (0, 1):
+        assert all(torch.equal(x, y) for run in got[i] for x, y in zip(run, want[i]))
+
+
+def test_one_tensor_for_all(device):
+    """q, k and v the same tensor: its gradient is the three together."""
+    q, _, _, g, b, cu, _ = case(device, torch.float32, 3, 32, [70, 9], seed=95)
+    x = q.clone().requires_grad_(True)
+    parts = [q.clone().requires_grad_(True) for _ in range(3)]
+    whole, = torch.autograd.grad(relative_attention(x, x, x, b, cu, cu), (x,), g)
+    split = torch.autograd.grad(relative_attention(*parts, b, cu, cu), parts, g)
+    assert float((whole - sum(split)).norm()) <= 2.0 ** -22 * sum(float(y.norm()) for y in split)
