@@ -15,6 +15,12 @@
 // frequency in turns; 32 would lose the angle of far positions) and its cosines
 // and sines wait in LDS.  A pair's other half of the half-split order is
 // fetched from the lane that holds it, four dims at a time.
+//
+// 129,850 tokens, 32 query and 32 key heads of 16 in bf16: forward 95 to 98 us
+// for 400 MB as counted at memory, backward 163 to 168 for 533 MB; 8 and 8 heads of 64
+// in fp32 (43,670 tokens): 67 to 69 us for 269 MB, 106 for 359; a copy reaches
+// 4.7 TB/s.  A call of one graph is one launch of 7 us, most of it the latency of
+// the 64-bit angles.
 #include <algorithm>
 
 #include "esa_common.h"

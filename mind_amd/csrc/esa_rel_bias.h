@@ -5,8 +5,11 @@
 // The preparation pass writes the table out by distance: per head a line of
 // bias * log2(e) at entry d + reach + kRelPad.  From `reach` (the distance at
 // which a side's last bucket begins) on the bias is constant, so only tiles
-// that cross |d| < reach read the line (from LDS, one entry per score); every
-// other tile has one value, which the exponent's FMA takes for free.
+// that cross |d| < reach differ within themselves.  Scores take the line's
+// entries (from LDS, one per score) as their matrix product's seed or in the
+// exponent's FMA.  The bf16 forward and dQ pass give the other tiles their one
+// value (it moves the forward's reference point: no operation per score); the
+// others read it from the line's pads.
 //
 // The table's gradient sums dS over the pairs of a bucket, in a fixed order
 // and without atomics.  In the dQ pass a wave's dS of a stage (64 keys by its
@@ -20,6 +23,19 @@
 // sums the blocks.  (By ds_add_f32, one per score, into a ring of distances per
 // wave, about 160 cycles an instruction, the dQ pass took 6.2 ms instead of 2.0
 // at 129,850 tokens, 32 heads of 16.)
+//
+// Vector instructions bound it: at those sizes forward, dQ and dK/dV take 0.94,
+// 1.53 and 1.58 ms at best (0.81, 1.12 and 1.36 without a bias), their vector
+// pipes busy 62, 78 and 70 % of the time and their matrix pipes 32, 24 and
+// 27 %; one exponential a score is 31, 19 and 18 %.  A near stage of dQ spends 96
+// instructions on the diagonals beside some 210 on its two tiles.
+//
+// bf16 calls round P and dS to bf16 where they are operands of the products over
+// keys and queries, as the kernels without a bias do: gradients 2.4 to 2.5e-3 of
+// their norm off, 1.7e-3 of it their own last rounding.  Sums of dS and the row
+// statistics are of unrounded values.  (P V with P's residue in a second product
+// made the output and the table's gradient exact to their last rounding and dq
+// 2.46 instead of 2.50e-3, for 1.61 ms instead of 0.94.)
 #pragma once
 #include <hip/hip_runtime.h>
 
