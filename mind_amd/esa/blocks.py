@@ -137,7 +137,7 @@ def _stand_in(setup, d, params, seeds=None):
     blk = SimpleNamespace(idx=1 if setup.mask else 0, use_mlp=setup.n_mlp > 0, residual_dropout=0.0,
                           norm=norm(setup.eps[0]))
     mab = SimpleNamespace(fc_q=linear(), fc_k=linear(), fc_v=linear(), fc_o=linear(), num_heads=setup.heads, dim_V=d,
-                          dropout_p=setup.dropout[0], training=True)
+                          order=None, dropout_p=setup.dropout[0], training=True)
     blk.sab = blk.pma = SimpleNamespace(mab=mab, S=seeds)
     if setup.n_mlp:
         blk.norm_mlp = norm(setup.eps[1])
