@@ -276,14 +276,14 @@ DEVI void wait_vmcnt() {
 // segment of n tokens either way.
 constexpr int kPlanBuckets = 1024;
 
-// `shift`, where given, gets for each group shift_of(segment).
-struct NoShift {
-  DEVI int operator()(int) const { return 0; }
+// note(i, s, j) is called for the j-th group of segment s, listed as i-th.
+struct NoNote {
+  DEVI void operator()(int, int, int) const {}
 };
-template <class ShiftOf = NoShift>
+template <class Note = NoNote>
 DEVI void seg_plan_block(const int* __restrict__ cu_outer, const int* __restrict__ cu_inner, int nseg, int gtok,
                          int4* __restrict__ groups, int* __restrict__ count, int tid, bool pairs = false,
-                         int* __restrict__ shift = nullptr, ShiftOf shift_of = ShiftOf()) {
+                         Note note = Note()) {
   constexpr int PER = kPlanBuckets / 256;
   __shared__ int hist[kPlanBuckets];
   __shared__ int part[256];
@@ -325,8 +325,7 @@ DEVI void seg_plan_block(const int* __restrict__ cu_outer, const int* __restrict
     const int pos = atomicAdd(&hist[bucket(s)], ng);
     const int ib = cu_inner[s], ie = cu_inner[s + 1];
     for (int j = 0; j < ng; ++j) groups[pos + j] = make_int4(max(ob, base + j * gtok), oe, ib, max(ie, ib));
-    if (shift)
-      for (int j = 0; j < ng; ++j) shift[pos + j] = shift_of(s);
+    for (int j = 0; j < ng; ++j) note(pos + j, s, j);
   }
 }
 

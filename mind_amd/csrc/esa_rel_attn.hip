@@ -75,7 +75,7 @@ size_t split_most(int batch, int total_q, int total_k, int keys) {
   return (size_t)(total_q + kSplitRows - 1) / kSplitRows + (size_t)(total_k + keys - 1) / keys + 2 * (size_t)batch;
 }
 
-struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, line, top, ranges, knorm, rows, part, where, acc, ml, total; };
+struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, first_q, slot_q, line, top, ranges, knorm, rows, part, where, acc, ml, total; };
 Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int buckets, int reach, int dtype, bool backward) {
   Layout w{};
   size_t off = 0;
@@ -98,6 +98,8 @@ Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int 
   if (backward) {
     w.plan_k = take(gk * sizeof(int4));
     w.shift_k = take(gk * sizeof(int));
+    w.first_q = take((size_t)batch * sizeof(int));
+    w.slot_q = take(gq * sizeof(int));
     w.rows = take((size_t)heads * tiles32(total_q) * kTile * sizeof(float2));
     w.part = take(gq * heads * buckets * sizeof(float));
   } else if (dtype == ESA_BF16) {
@@ -156,6 +158,8 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
   if (backward) {
     r.plan_k = reinterpret_cast<int4*>(at(w.plan_k));
     r.shift_k = reinterpret_cast<int*>(at(w.shift_k));
+    r.first_q = reinterpret_cast<int*>(at(w.first_q));
+    r.bias.slot = r.slot_q = reinterpret_cast<int*>(at(w.slot_q));
     r.rows = reinterpret_cast<float2*>(at(w.rows));
   } else if (dtype == ESA_BF16) {
     if ((r.split.keys = split_keys(c.nseg, c.total_q, c.total_k, c.heads, dtype, false))) {

@@ -53,7 +53,8 @@ struct RelBias {
   const int2* ranges;       // [buckets] entries [x, y) of the line
   int reach, stride;        // stride = 2 (reach + kRelPad) + 1
   int buckets, far_lo, far_hi;   // the buckets of d <= -reach and d >= reach
-  float* part;              // dQ pass: [groups][heads][buckets]
+  float* part;              // dQ pass: [groups][heads][buckets], the groups in their tokens' order
+  const int* slot;          // dQ pass: a listed group's place in that order
 };
 
 // Few queries over many keys (bf16 forward): a group is 32 queries of one
@@ -81,6 +82,7 @@ struct RelPass {
   int4* plan_q; int4* plan_k;       // groups of 128 or 64 tokens (seg_plan_block); plan_k backward only
   int* count_q; int* count_k;
   int* shift_q; int* shift_k;       // per group: d = key token - query token - shift
+  int* first_q; int* slot_q;        // backward: a segment's first place, a listed group's place in the tokens' order
   float* knorm; int tk_tiles;       // bf16 forward: max |k| per (head, 32-key tile)
   float2* rows; int tq_pad;         // backward: row statistics [heads][tq_pad]
   RelSplit split;                   // bf16 forward of few queries
@@ -331,6 +333,30 @@ DEVI void split_plan_block(const RelPrep& p, const RelPass& r, int tid, ShiftOf 
   }
 }
 
+// first[s] = groups of the segments before s.  The plan lists groups of equal work in any order; the table's partial sums
+// are added in this one.
+DEVI void seg_first_block(const int* cu, int nseg, int gtok, int* first, int tid) {
+  __shared__ int part[256];
+  const int per = (nseg + 255) / 256, s0 = min(tid * per, nseg), s1 = min(s0 + per, nseg);
+  auto groups = [&](int s) { return max(cu[s + 1] - cu[s] + gtok - 1, 0) / gtok; };
+  int sum = 0;
+  for (int s = s0; s < s1; ++s) sum += groups(s);
+  part[tid] = sum;
+  __syncthreads();
+  for (int off = 1; off < 256; off <<= 1) {
+    const int add = tid >= off ? part[tid - off] : 0;
+    __syncthreads();
+    part[tid] += add;
+    __syncthreads();
+  }
+  int at = part[tid] - sum;
+  for (int s = s0; s < s1; ++s) {
+    first[s] = at;
+    at += groups(s);
+  }
+  __syncthreads();
+}
+
 // Block b of the preparation's rel_prep_blocks (256 threads).
 DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
   auto shift_of = [&](int s) {
@@ -342,13 +368,18 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
     return;
   }
   if (b == 0) {
-    seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, r.shift_q, shift_of);
+    if (p.backward) seg_first_block(p.cu_q, p.nseg, p.gtok_q, r.first_q, tid);
+    seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, [&](int i, int s, int j) {
+      r.shift_q[i] = shift_of(s);
+      if (p.backward) r.slot_q[i] = r.first_q[s] + j;
+    });
     return;
   }
   b -= 1;
   if (p.backward) {
     if (b == 0) {
-      seg_plan_block(p.cu_k, p.cu_q, p.nseg, p.gtok_k, r.plan_k, r.count_k, tid, p.key_pairs, r.shift_k, shift_of);
+      seg_plan_block(p.cu_k, p.cu_q, p.nseg, p.gtok_k, r.plan_k, r.count_k, tid, p.key_pairs,
+                     [&](int i, int s, int) { r.shift_k[i] = shift_of(s); });
       return;
     }
     b -= 1;

@@ -460,3 +460,12 @@ def test_one_tensor_for_all(device):
     whole, = torch.autograd.grad(relative_attention(x, x, x, b, cu, cu), (x,), g)
     split = torch.autograd.grad(relative_attention(*parts, b, cu, cu), parts, g)
     assert float((whole - sum(split)).norm()) <= 2.0 ** -22 * sum(float(y.norm()) for y in split)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 16), (torch.bfloat16, 32), (torch.float32, 16)])
+def test_table_gradient_of_many_equal_segments(device, dtype, hd):
+    """Segments of equal length are planned in any order; the table's gradient adds them in the tokens'."""
+    q, k, v, g, b, cu, _ = case(device, dtype, 2, hd, [33] * 900 + [0, 170] * 40, seed=97)
+    leaves = [x.requires_grad_(True) for x in (q, k, v, b)]
+    grads = [torch.autograd.grad(relative_attention(*leaves, cu, cu), leaves, g) for _ in range(6)]
+    assert all(torch.equal(x, y) for run in grads[1:] for x, y in zip(run, grads[0]))
