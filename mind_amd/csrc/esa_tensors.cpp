@@ -5,9 +5,10 @@
 // (pointer, count, dtype, layout, device) in one pass, and says whether the
 // written ones share memory (a dozen properties of 768 gradients and their
 // targets took 650 us, here 15 us).
-// Forwards of small batches, whose kernels take 10 us: the checks of a call's
+// Calls over small batches, whose kernels take 10 us: the checks of a call's
 // arguments, its outputs and workspace and the call of the C entry in one
-// function each (the Python form of both together took 15 to 20 us a call).
+// function each (with their Python form a forward took 21 to 25 us of
+// host time, now 8 to 12; the body of a small backward 46, now 30).
 // The Python callers keep the checks' messages: a check here only says whether
 // there is anything to look at.
 #define PY_SSIZE_T_CLEAN
@@ -211,7 +212,7 @@ PyObject* changed(PyObject*, PyObject* list) {
   });
 }
 
-// ---- forwards
+// ---- calls of small batches
 
 // What the checks say of a call: its arguments fit, all tensors are of torch's own types, one wants a gradient.
 constexpr long kFits = 1, kExact = 2, kGrad = 4;
@@ -291,6 +292,10 @@ int without_gil(F f) {
   Py_END_ALLOW_THREADS return rc;
 }
 
+at::Tensor bytes_on(const at::Tensor& like, size_t bytes) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 256)}, like.options().dtype(at::kByte));
+}
+
 // relative_forward(address of esa_rel_attn_fwd, of its size query, stream, q, k, v, bias, starts (bytes of int32), q_start,
 // cu_q, cu_k, scale, dropout_p, seed, keep) -> (status, out, out_low or None, lse, the table); keep: out_low is wanted.
 PyObject* relative_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -320,7 +325,7 @@ PyObject* relative_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
       out = at::empty(q.sizes(), q.options());
       if (keep) low = at::empty(q.sizes(), q.options());
       lse = at::empty({heads, tq}, q.options().dtype(at::kFloat));
-      ws = at::empty({(int64_t)std::max<size_t>(bytes, 256)}, q.options().dtype(at::kByte));
+      ws = bytes_on(q, bytes);
       rc = without_gil([&] {
         return fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), code_of(table), buckets, starts, side, q_start,
                   cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), batch, tq, tk, heads, hd, code_of(q), scale, dropout, seed,
@@ -329,6 +334,55 @@ PyObject* relative_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
       });
     }
     return tuple_of({PyLong_FromLong(rc), wrapped(out), wrapped(low), wrapped(lse), wrapped(table)});
+  });
+}
+
+// A gradient as the kernels take it: dense, by value, on a 16-byte boundary.
+at::Tensor gradient_of(PyObject* o) {
+  const at::Tensor g = tensor_of(o).resolve_neg().contiguous();
+  return reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 ? g.clone() : g;
+}
+
+// relative_backward(address of esa_rel_attn_bwd, of its size query, stream, dout, q, k, v, out, out_low, lse, table, starts,
+// q_start, cu_q, cu_k, scale, dropout_p, seed) -> (status, dq, dk, dv, dtable in the table's type); arguments as the
+// forward's and its results
+PyObject* relative_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 18 && PyBytes_Check(args[11]), "relative_backward: arguments");
+    const auto fn = reinterpret_cast<decltype(&esa_rel_attn_bwd)>(PyLong_AsVoidPtr(args[0]));
+    const auto size_of = reinterpret_cast<decltype(&esa_rel_attn_workspace_size)>(PyLong_AsVoidPtr(args[1]));
+    void* stream = PyLong_AsVoidPtr(args[2]);
+    const at::Tensor &q = tensor_of(args[4]), &k = tensor_of(args[5]), &v = tensor_of(args[6]), &out = tensor_of(args[7]);
+    const void* low = pointer_of(args[8]);
+    const at::Tensor &lse = tensor_of(args[9]), &table = tensor_of(args[10]);
+    const int* starts = reinterpret_cast<const int*>(PyBytes_AS_STRING(args[11]));
+    const int side = (int)(PyBytes_GET_SIZE(args[11]) / sizeof(int)), buckets = (int)table.size(0);
+    const int* q_start = static_cast<const int*>(pointer_of(args[12]));
+    const at::Tensor &cu_q = tensor_of(args[13]), &cu_k = tensor_of(args[14]);
+    const float scale = (float)PyFloat_AsDouble(args[15]), dropout = (float)PyFloat_AsDouble(args[16]);
+    const unsigned long long seed = PyLong_AsUnsignedLongLong(args[17]);
+    if (PyErr_Occurred()) return nullptr;
+    const int batch = (int)cu_q.numel() - 1, tq = (int)q.size(0), tk = (int)k.size(0), heads = (int)q.size(1), hd = (int)q.size(2);
+    const c10::DeviceGuard on(q.device());
+    const at::Tensor g = gradient_of(args[3]);
+    at::Tensor dq, dk, dv, dtable;
+    size_t bytes = 0;
+    int rc = size_of(batch, tq, tk, heads, hd, code_of(q), buckets, starts, side, 1, &bytes);
+    if (rc == ESA_OK) {
+      dq = at::empty(q.sizes(), q.options());
+      dk = at::empty(k.sizes(), k.options());
+      dv = at::empty(v.sizes(), v.options());
+      dtable = at::empty(table.sizes(), table.options().dtype(at::kFloat));
+      const at::Tensor ws = bytes_on(q, bytes);
+      rc = without_gil([&] {
+        return fn(g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low, lse.data_ptr<float>(),
+                  table.data_ptr(), code_of(table), buckets, starts, side, q_start, cu_q.data_ptr<int>(), cu_k.data_ptr<int>(),
+                  batch, tq, tk, heads, hd, code_of(q), scale, dropout, seed, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  dtable.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream);
+      });
+      if (rc == ESA_OK && table.scalar_type() != at::kFloat) dtable = dtable.to(table.scalar_type());
+    }
+    return tuple_of({PyLong_FromLong(rc), wrapped(dq), wrapped(dk), wrapped(dv), wrapped(dtable)});
   });
 }
 
@@ -448,10 +502,64 @@ PyObject* qk_norm_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// qk_norm_backward(address of esa_qk_norm_bwd, of its size query, stream, gq, gk, q, k, wq, wk, positions, frequencies, eps,
+// interleaved, type code of dwq or None, of dwk) -> (status, dq, dk or None, dwq or None, dwk or None); q and k the rows
+// that the forward returned; type codes: ESA_F32, ESA_BF16
+PyObject* qk_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 15, "qk_norm_backward: arguments");
+    const auto fn = reinterpret_cast<decltype(&esa_qk_norm_bwd)>(PyLong_AsVoidPtr(args[0]));
+    const auto size_of = reinterpret_cast<decltype(&esa_qk_norm_bwd_workspace_size)>(PyLong_AsVoidPtr(args[1]));
+    void* stream = PyLong_AsVoidPtr(args[2]);
+    const at::Tensor& q = tensor_of(args[5]);
+    const bool keys = args[6] != Py_None;
+    const at::Tensor& k = keys ? tensor_of(args[6]) : q;
+    const float *wq = static_cast<const float*>(pointer_of(args[7])), *wk = static_cast<const float*>(pointer_of(args[8]));
+    const void* positions = pointer_of(args[9]);
+    const int positions_bytes = args[9] != Py_None ? (int)tensor_of(args[9]).element_size() : 0;
+    const double* frequencies = static_cast<const double*>(pointer_of(args[10]));
+    const int rotary = args[10] != Py_None ? 2 * (int)tensor_of(args[10]).numel() : 0;
+    const float eps = (float)PyFloat_AsDouble(args[11]);
+    const int interleaved = PyObject_IsTrue(args[12]);
+    const long code[2] = {args[13] == Py_None ? -1 : PyLong_AsLong(args[13]), args[14] == Py_None ? -1 : PyLong_AsLong(args[14])};
+    if (PyErr_Occurred()) return nullptr;
+    const long long strides[4] = {q.stride(0), q.stride(1), keys ? k.stride(0) : 0, keys ? k.stride(1) : 0};
+    const int total = (int)q.size(0), hd = (int)q.size(2);
+    const c10::DeviceGuard on(q.device());
+    const at::Tensor gq = gradient_of(args[3]), dq = at::empty(q.sizes(), q.options());
+    at::Tensor gk, dk, dw[2], ws;
+    if (keys) {
+      gk = gradient_of(args[4]);
+      dk = at::empty(k.sizes(), k.options());
+    }
+    int rc = ESA_OK;
+    for (int i = 0; i < 2; ++i)
+      if (code[i] >= 0) dw[i] = at::empty({hd}, q.options().dtype(at::kFloat));
+    if (dw[0].defined() || dw[1].defined()) {
+      size_t bytes = 0;
+      rc = size_of(total, hd, &bytes);
+      if (rc == ESA_OK) ws = bytes_on(q, bytes);
+    }
+    if (rc == ESA_OK)
+      rc = without_gil([&] {
+        return fn(gq.data_ptr(), keys ? gk.data_ptr() : nullptr, q.data_ptr(), keys ? k.data_ptr() : nullptr, strides, total,
+                  (int)q.size(1), keys ? (int)k.size(1) : 0, hd, code_of(q), wq, wk, positions, positions_bytes, frequencies,
+                  rotary, interleaved, eps, dq.data_ptr(), keys ? dk.data_ptr() : nullptr,
+                  dw[0].defined() ? dw[0].data_ptr<float>() : nullptr, dw[1].defined() ? dw[1].data_ptr<float>() : nullptr,
+                  ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream);
+      });
+    for (int i = 0; i < 2; ++i)
+      if (rc == ESA_OK && code[i] == kBf16) dw[i] = dw[i].to(at::kBFloat16);
+    return tuple_of({PyLong_FromLong(rc), wrapped(dq), wrapped(dk), wrapped(dw[0]), wrapped(dw[1])});
+  });
+}
+
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)); }
 
 PyMethodDef methods[] = {{"relative_fits", fast(relative_fits), METH_FASTCALL, nullptr},
                          {"relative_forward", fast(relative_forward), METH_FASTCALL, nullptr},
+                         {"relative_backward", fast(relative_backward), METH_FASTCALL, nullptr},
+                         {"qk_norm_backward", fast(qk_norm_backward), METH_FASTCALL, nullptr},
                          {"qk_norm_fits", fast(qk_norm_fits), METH_FASTCALL, nullptr},
                          {"qk_norm_forward", fast(qk_norm_forward), METH_FASTCALL, nullptr},
                          {"clip", fast(clip), METH_FASTCALL, nullptr},

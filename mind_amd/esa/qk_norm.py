@@ -7,7 +7,6 @@ the token's position.  The reference has no counterpart: its layers see a set.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -17,7 +16,6 @@ from .. import _lib
 from .attention import HEAD_DIMS
 from .eager import FITS, call_checked
 from .layer_norm import f32_values
-from .linear import on_boundary
 
 _CODES = {torch.float32: _lib.ESA_F32, torch.bfloat16: _lib.ESA_BF16}
 MAX_HEADS = 2048
@@ -28,18 +26,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> t
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive (got {rotary_dim})")
     return float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
-
-
-def _strides(q, k):
-    return (ctypes.c_longlong * 4)(q.stride(0), q.stride(1), *((0, 0) if k is None else (k.stride(0), k.stride(1))))
-
-
-def _common(q, k, wq, wk, positions, frequencies, interleaved, eps):
-    """The C ABI's arguments from `total` to eps."""
-    turned = frequencies is not None
-    return (q.shape[0], q.shape[1], 0 if k is None else k.shape[1], q.shape[2], _CODES[q.dtype], _lib.ptr(wq), _lib.ptr(wk),
-            _lib.ptr(positions), positions.element_size() if turned else 0, _lib.ptr(frequencies),
-            2 * frequencies.numel() if turned else 0, int(interleaved), eps)
 
 
 class _QkNorm(torch.autograd.Function):
@@ -59,23 +45,11 @@ class _QkNorm(torch.autograd.Function):
     def backward(ctx, gq, gk=None):
         q, k, wq, wk, positions, frequencies = ctx.saved_tensors
         eps, interleaved = ctx.meta
-        gq, gk = on_boundary(gq.contiguous()), None if k is None else on_boundary(gk.contiguous())
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dws = [torch.empty(q.shape[2], dtype=torch.float32, device=q.device) if n else None for n in ctx.needs_input_grad[2:4]]
-        lib, ws = _lib.load(), None
-        with _lib.on_device(q):
-            if any(w is not None for w in dws):
-                n = ctypes.c_size_t(0)
-                _lib.check(lib.esa_qk_norm_bwd_workspace_size(q.shape[0], q.shape[2], ctypes.byref(n)),
-                           "esa_qk_norm_bwd_workspace_size")
-                ws = torch.empty(max(int(n.value), 256), dtype=torch.uint8, device=q.device)
-            _lib.check(lib.esa_qk_norm_bwd(
-                gq.data_ptr(), _lib.ptr(gk), q.data_ptr(), _lib.ptr(k), _strides(q, k),
-                *_common(q, k, wq, wk, positions, frequencies, interleaved, eps), dq.data_ptr(), _lib.ptr(dk),
-                _lib.ptr(dws[0]), _lib.ptr(dws[1]), _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q)),
-                "esa_qk_norm_bwd")
-        dwq, dwk = (w if w is None else w.to(t) for w, t in zip(dws, ctx.weight_dtypes))
+        wanted = [_CODES[t] if n else None for n, t in zip(ctx.needs_input_grad[2:4], ctx.weight_dtypes)]
+        rc, dq, dk, dwq, dwk = _lib.tensors().qk_norm_backward(
+            _lib.address("esa_qk_norm_bwd"), _lib.address("esa_qk_norm_bwd_workspace_size"), _lib.stream_of(q), gq, gk, q, k, wq, wk,
+            positions, frequencies, eps, interleaved, *wanted)
+        _lib.check(rc, "esa_qk_norm_bwd")
         return dq, dk, dwq, dwk, None, None, None, None
 
 

@@ -16,12 +16,11 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .attention import (_SEED_MASK, _check_dropout, _check_index, _check_tokens, _dtype_code, draw_dropout_seed)
+from .attention import _SEED_MASK, _check_dropout, _check_index, _check_tokens, draw_dropout_seed
 from .eager import FITS, call_checked
-from .linear import on_boundary
 
 MAX_REACH, MAX_BUCKETS = 768, 256
-_TABLE = {torch.float32: _lib.ESA_F32, torch.bfloat16: _lib.ESA_BF16}
+_TABLE = (torch.float32, torch.bfloat16)
 
 
 @functools.lru_cache(maxsize=64)
@@ -81,23 +80,11 @@ class _RelativeAttention(torch.autograd.Function):
         if g is None:
             return (None,) * 11
         starts, scale, dropout_p, seed = ctx.meta
-        (tq, heads, hd), tk, batch, dt = q.shape, k.shape[0], cu_q.numel() - 1, _dtype_code(q)
-        g = on_boundary(g.contiguous())
-        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        dtable = torch.empty(table.shape, dtype=torch.float32, device=q.device)
-        c_starts = (ctypes.c_int * len(starts))(*starts)
-        with _lib.on_device(q):
-            need = ctypes.c_size_t(0)
-            _lib.check(_lib.load().esa_rel_attn_workspace_size(batch, tq, tk, heads, hd, dt, table.shape[0], c_starts,
-                                                               len(starts), 1, ctypes.byref(need)),
-                       "esa_rel_attn_workspace_size")
-            ws = torch.empty(max(int(need.value), 256), dtype=torch.uint8, device=q.device)
-            _lib.check(_lib.load().esa_rel_attn_bwd(
-                g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(low), lse.data_ptr(),
-                table.data_ptr(), _TABLE[table.dtype], table.shape[0], c_starts, len(starts), _lib.ptr(q_start), cu_q.data_ptr(),
-                cu_k.data_ptr(), batch, tq, tk, heads, hd, dt, scale, dropout_p, seed, dq.data_ptr(), dk.data_ptr(),
-                dv.data_ptr(), dtable.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(q)), "esa_rel_attn_bwd")
-        return dq, dk, dv, dtable.to(table.dtype), None, None, None, None, None, None, None
+        rc, dq, dk, dv, dtable = _lib.tensors().relative_backward(
+            _lib.address("esa_rel_attn_bwd"), _lib.address("esa_rel_attn_workspace_size"), _lib.stream_of(q), g, q, k, v, out, low,
+            lse, table, _start_bytes(starts), q_start, cu_q, cu_k, scale, dropout_p, seed)
+        _lib.check(rc, "esa_rel_attn_bwd")
+        return dq, dk, dv, dtable, None, None, None, None, None, None, None
 
 
 def _check(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start):
