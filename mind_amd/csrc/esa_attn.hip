@@ -1426,21 +1426,21 @@ DEVI f32x4 mfma16x4f(float a, float b, const f32x4& c) { return __builtin_amdgcn
 // The stage's rows of a [T][H][HD] tensor from token t0 on, into registers and from there into LDS; tokens at or
 // past `end` are zeros, or with REPEAT the last row again.
 template <class T, bool REPEAT = false>
-DEVI void f32_load(f32x4 (&r)[T::kPer], const float* src, int end, int H, int head, int t0) {
+DEVI void f32_load(f32x4 (&r)[T::kPer], const float* src, int end, int H, int head, int t0, unsigned tid = threadIdx.x) {
   constexpr int HD = T::kHd;
 #pragma unroll
   for (int i = 0; i < T::kPer; ++i) {
-    const int x = threadIdx.x + i * T::kThreads, part = x % (4 * T::NR);
+    const int x = tid + i * T::kThreads, part = x % (4 * T::NR);
     const int t = REPEAT ? min(t0 + x / (4 * T::NR), end - 1) : t0 + x / (4 * T::NR);
     r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (t < end && part < HD / 4) r[i] = *reinterpret_cast<const f32x4*>(src + ((size_t)t * H + head) * HD + 4 * part);
   }
 }
 template <class T>
-DEVI void f32_store(float (*dst)[T::kStride], const f32x4 (&r)[T::kPer]) {
+DEVI void f32_store(float (*dst)[T::kStride], const f32x4 (&r)[T::kPer], unsigned tid = threadIdx.x) {
 #pragma unroll
   for (int i = 0; i < T::kPer; ++i) {
-    const int x = threadIdx.x + i * T::kThreads;
+    const int x = tid + i * T::kThreads;
     *reinterpret_cast<f32x4*>(&dst[x / (4 * T::NR)][4 * (x % (4 * T::NR))]) = r[i];
   }
 }
@@ -1596,19 +1596,43 @@ DEVI void f32_stages(int lo, int hi, bool live, Load load, Store store, Use use)
   }
 }
 
+// The same by two halves of a block's waves, which take the stages in turn: `load(t0)` of the half's own stage, `use` where
+// it lies in the range.
+template <class Load, class Store, class Use>
+DEVI void f32_stages_halved(int lo, int hi, int half, bool live, Load load, Store store, Use use) {
+  if (lo >= hi) return;
+  const int mine = kF32Stage * half;
+  load(lo + mine);
+  store(0);
+  int buf = 0;
+  for (int t0 = lo; t0 < hi; t0 += 2 * kF32Stage, buf ^= 1) {
+    const bool more = t0 + 2 * kF32Stage < hi;   // block-uniform
+    if (more) load(t0 + 2 * kF32Stage + mine);
+    __syncthreads();
+    if (live && t0 + mine < hi) use(buf, t0 + mine);
+    if (more) store(buf ^ 1);
+  }
+}
+
 // With a bias, head dims 24 and 32 spill a dozen registers at four waves a SIMD; at three they take 2 to 5 % less time
 // (600 segments of 60 tokens, 8 heads of 24 dims: 67 against 71 us).
-template <bool MASKED, int HD, bool DROP, bool BIAS = false, int TOK = kGroupTok>
-__global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_per_eu(
+// HALVES 2: twice the waves, both halves with the group's queries and every second stage of keys, joined at the end.
+template <bool MASKED, int HD, bool DROP, bool BIAS = false, int TOK = kGroupTok, int HALVES = 1>
+__global__ __launch_bounds__(HALVES* f32_threads(HD, TOK)) __attribute__((amdgpu_waves_per_eu(
     MASKED ? 1 : BIAS && (HD == 24 || HD == 32) ? 3 : 4))) void attn_fwd_f32_kernel(const AttnF32Args a) {
   using T = F32Tile<HD, TOK>;
   constexpr int NR = T::NR, QB = T::QB, KB = kF32Stage / 16;
-  __shared__ __align__(16) typename T::Rows sK[2], sV[2];
+  __shared__ __align__(16) typename T::Rows sKs[HALVES][2], sVs[HALVES][2];
   __shared__ int2 sN[2][MASKED ? kF32Stage : 1];
-  __shared__ uint32_t sKey[2][DROP ? kF32Stage : 1];   // column keys of the staged keys
+  __shared__ uint32_t sKeys[HALVES][2][DROP ? kF32Stage : 1];   // column keys of the staged keys
   const int H = a.heads, item = blockIdx.x / H, head = blockIdx.x - item * H;
   if (item >= *a.count) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave_all = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int half = HALVES == 2 ? wave_all / (T::kThreads / 64) : 0, wave = HALVES == 2 ? wave_all % (T::kThreads / 64) : wave_all;
+  const int tid = HALVES == 2 ? wave * 64 + lane : (int)threadIdx.x;
+  auto& sK = sKs[half];
+  auto& sV = sVs[half];
+  auto& sKey = sKeys[half];
   const int c16 = lane & 15, grp = lane >> 4;
   const F32Own<HD, QB> own(a.plan[item], wave, c16);
   const int phi = own.phi;
@@ -1627,25 +1651,23 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
     l[b] = 0.f;
   }
   const int first = a.plan[item].x + 16 * QB * wave, shift = BIAS ? a.shift[item] : 0;
-  if (BIAS) rel_load_line<T::kThreads>(sRel, a.rel, head, tid);
+  if (BIAS) rel_load_line<HALVES * T::kThreads>(sRel, a.rel, head, threadIdx.x);
   f32x4 rK[T::kPer], rV[T::kPer];
   int2 rN = make_int2(-1, -1);
   uint32_t rKey = 0;
-  f32_stages(
-      own.plo, phi, own.live,
-      [&](int t0) {
-        f32_load<T>(rK, a.k, phi, H, head, t0);
-        f32_load<T>(rV, a.v, phi, H, head, t0);
+  auto load = [&](int t0) {
+        f32_load<T>(rK, a.k, phi, H, head, t0, HALVES == 2 ? (unsigned)tid : threadIdx.x);
+        f32_load<T>(rV, a.v, phi, H, head, t0, HALVES == 2 ? (unsigned)tid : threadIdx.x);
         if (MASKED && tid < kF32Stage) rN = t0 + tid < phi ? a.nodes[t0 + tid] : make_int2(-1, -1);
         if (DROP && tid < kF32Stage) rKey = drop_col(a.drop, t0 + tid);
-      },
-      [&](int buf) {
-        f32_store<T>(sK[buf], rK);
-        f32_store<T>(sV[buf], rV);
+      };
+  auto store = [&](int buf) {
+        f32_store<T>(sK[buf], rK, HALVES == 2 ? (unsigned)tid : threadIdx.x);
+        f32_store<T>(sV[buf], rV, HALVES == 2 ? (unsigned)tid : threadIdx.x);
         if (MASKED && tid < kF32Stage) sN[buf][tid] = rN;
         if (DROP && tid < kF32Stage) sKey[buf][tid] = rKey;
-      },
-      [&](int buf, int k0) {
+      };
+  auto use = [&](int buf, int k0) {
         f32x4 s[KB][QB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -1708,7 +1730,34 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
             }
         }
         f32_add_stage<HD>(acc, sV[buf], s, c16, grp);
-      });
+      };
+  if constexpr (HALVES == 1) {
+    f32_stages(own.plo, phi, own.live, load, store, use);
+  } else {
+    f32_stages_halved(own.plo, phi, half, own.live, load, store, use);
+    static_assert(HALVES == 1 || (QB == 1 && sizeof(sKs) >= (4 * NR + 2) * T::kThreads * sizeof(float)), "");
+    float* other = reinterpret_cast<float*>(sKs) + tid;   // the second half's values, one run of threads each
+    constexpr int W = T::kThreads;
+    __syncthreads();
+    if (half == 1) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) other[(4 * c + e) * W] = acc[0][c][e];
+      other[4 * NR * W] = m[0];
+      other[(4 * NR + 1) * W] = l[0];
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float m2 = other[4 * NR * W], top = fmaxf(m[0], m2);
+    const float x = m[0] == -INFINITY ? 0.f : fast_exp2(m[0] - top), y = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top);
+    l[0] = l[0] * x + other[(4 * NR + 1) * W] * y;
+#pragma unroll
+    for (int c = 0; c < NR; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][c][e] = acc[0][c][e] * x + other[(4 * c + e) * W] * y;
+    m[0] = top;
+  }
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     float sum = l[b] + __shfl_xor(l[b], 16);
@@ -2796,6 +2845,24 @@ int scratch_address(void** out) {
 
 }  // namespace
 
+// Two halves of waves a block, as long as the blocks leave room for them: the walk of the longest segment is half as long.
+// Forward of 8 heads of 16 with 288 blocks 21.1 -> 18.0 us, 1,072: 40.6 -> 38.1, 1,576: 51.3 -> 48.4, 3,232: 83.5 -> 84.9; of 32:
+// 288: 27.8 -> 23.7, 1,072: 59.0 -> 55.5, 1,576: 74.0 -> 75.1; 16 heads of 24 with 576: 33.5 -> 32.9, 2,144: 97 -> 102.  Head
+// dim 64 has no LDS for both halves' stages.
+bool f32_rel_halved(dim3 grid, int head_dim, int tok) {
+  return tok == kFewTok && head_dim < 64 && grid.x <= (head_dim == 16 ? 2048u : 1280u);
+}
+template <bool D, int HD>
+void f32_rel_fwd_halved_hd(dim3 grid, size_t lds, hipStream_t st, const AttnF32Args& a) {
+  hipLaunchKernelGGL((attn_fwd_f32_kernel<false, HD, D, true, kFewTok, 2>), grid, dim3(2 * f32_threads(HD, kFewTok)), lds, st, a);
+}
+template <bool D>
+void f32_rel_fwd_halved(int hd, dim3 grid, size_t lds, hipStream_t st, const AttnF32Args& a) {
+  if (hd == 16) f32_rel_fwd_halved_hd<D, 16>(grid, lds, st, a);
+  else if (hd == 24) f32_rel_fwd_halved_hd<D, 24>(grid, lds, st, a);
+  else f32_rel_fwd_halved_hd<D, 32>(grid, lds, st, a);
+}
+
 int f32_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipStream_t st) {
   const int nb = rel_prep_blocks(p);
   ESA_TIMED(esa_profile::kAttnPrep, st,
@@ -2805,8 +2872,14 @@ int f32_rel_fwd(const DenseAttnCall& c, const RelPass& r, const RelPrep& p, hipS
   AttnF32Args a = f32_rel_args(c, r);
   a.o = static_cast<float*>(c.out); a.lse_out = c.lse;
   auto lds = [&](int) { return r.bias.stride * sizeof(float); };
-  ESA_TIMED(esa_profile::kAttnFwd, st,
-            ESA_F32_REL_LAUNCH(attn_fwd_f32_kernel, c.head_dim, c.dropout, f32_rel_grid(c.total_q, c, r.group_tok), lds, st, a));
+  const dim3 grid = f32_rel_grid(c.total_q, c, r.group_tok);
+  if (f32_rel_halved(grid, c.head_dim, r.group_tok))
+    ESA_TIMED(esa_profile::kAttnFwd, st, {
+      if (c.dropout) f32_rel_fwd_halved<true>(c.head_dim, grid, r.bias.stride * sizeof(float), st, a);
+      else f32_rel_fwd_halved<false>(c.head_dim, grid, r.bias.stride * sizeof(float), st, a);
+    });
+  else
+    ESA_TIMED(esa_profile::kAttnFwd, st, ESA_F32_REL_LAUNCH(attn_fwd_f32_kernel, c.head_dim, c.dropout, grid, lds, st, a));
   ESA_LAUNCH_CHECK();
   return ESA_OK;
 }

@@ -469,3 +469,10 @@ def test_table_gradient_of_many_equal_segments(device, dtype, hd):
     leaves = [x.requires_grad_(True) for x in (q, k, v, b)]
     grads = [torch.autograd.grad(relative_attention(*leaves, cu, cu), leaves, g) for _ in range(6)]
     assert all(torch.equal(x, y) for run in grads[1:] for x, y in zip(run, grads[0]))
+
+
+@pytest.mark.parametrize("hd", [16, 24, 32])
+@pytest.mark.parametrize("dropout", [0.0, 0.2])
+def test_blocks_between_in_single_precision(device, hd, dropout):
+    """The fp32 kernels' groups of 64 tokens with more blocks than the forward's halved walk takes."""
+    check(device, torch.float32, 7, hd, [100] * 150, dropout=dropout, seed=67)
