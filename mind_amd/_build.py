@@ -5,7 +5,7 @@ Each ``csrc/*.hip`` file is compiled to an object with ``hipcc
 whose only exported symbols are the ``extern "C"`` entry points declared in
 ``include/esa_hip.h``.  Objects go to ``mind_amd/_build/`` and stay out of
 version control; the ``.so`` is built in-tree so it travels with the
-repository snapshot to a GPU box.  ``csrc/esa_tensors.cpp`` (reading lists of
+tree.  ``csrc/esa_tensors.cpp`` (reading lists of
 torch tensors) is host code against torch's and Python's headers.
 """
 from __future__ import annotations
@@ -66,8 +66,8 @@ def _build_tensors() -> None:
     src, tmp = CSRC / "esa_tensors.cpp", TENSORS.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
-           *(f"-I{p}" for p in include_paths()), str(src), "-o", str(tmp), *(f"-L{p}" for p in library_paths()),
-           "-ltorch_python", "-ltorch_cpu", "-lc10"]   # torch has loaded them by the time this module is
+           *(f"-I{p}" for p in include_paths()), "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", str(src), "-o", str(tmp), *(f"-L{p}" for p in library_paths()),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]   # torch has loaded them by the time this module is
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{proc.stderr}")

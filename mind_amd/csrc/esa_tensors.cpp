@@ -6,9 +6,9 @@
 // written ones share memory (a dozen properties of 768 gradients and their
 // targets took 650 us, here 15 us).
 // Calls over small batches, whose kernels take 10 us: the checks of a call's
-// arguments, its outputs and workspace and the call of the C entry in one
-// function each (with their Python form a forward took 21 to 25 us of
-// host time, now 8 to 12; the body of a small backward 46, now 30).
+// arguments, its outputs and workspace, the call of the C entry and its record
+// for autograd in one function each (in Python a forward took 21 to 25 us of
+// host time, now 8 to 12, a training call 123 to 134, now 82 to 88).
 // The Python callers keep the checks' messages: a check here only says whether
 // there is anything to look at.
 #define PY_SSIZE_T_CLEAN
@@ -16,12 +16,21 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <exception>
+#include <memory>
+#include <mutex>
+#include <string>
 #include <vector>
 
 #include "../../include/esa_hip.h"
@@ -35,6 +44,15 @@ template <class F>
 PyObject* guarded(F f) {
   try {
     return f();
+  } catch (const c10::OutOfMemoryError& e) {
+    if (!PyErr_Occurred()) {
+      PyObject* torch = PyImport_ImportModule("torch");
+      PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+      if (type) PyErr_SetString(type, e.what_without_backtrace());
+      Py_XDECREF(type);
+      Py_XDECREF(torch);
+    }
+    return nullptr;
   } catch (const std::exception& e) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
@@ -214,8 +232,8 @@ PyObject* changed(PyObject*, PyObject* list) {
 
 // ---- calls of small batches
 
-// What the checks say of a call: its arguments fit, all tensors are of torch's own types, one wants a gradient.
-constexpr long kFits = 1, kExact = 2, kGrad = 4;
+// What the checks say of a call: its arguments fit, all tensors are of torch's own types.
+constexpr long kFits = 1, kExact = 2;
 
 int code_of(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? kF32 : t.scalar_type() == at::kBFloat16 ? kBf16 : -1; }
 bool head_dim_ok(int64_t d) { return d == 16 || d == 24 || d == 32 || d == 64; }
@@ -231,7 +249,6 @@ struct Args {
     }
     const at::Tensor& t = THPVariable_Unpack(o);
     if (!THPVariable_CheckTypeExact(Py_TYPE(o))) flags &= ~kExact;
-    if (t.requires_grad()) flags |= kGrad;
     if (!first) first = &t;
     if (t.layout() != at::kStrided || t.is_neg() || !t.is_cuda() || t.get_device() != first->get_device()) flags &= ~kFits;
     return &t;
@@ -285,104 +302,229 @@ PyObject* tuple_of(PyObject* const (&items)[N]) {
   return r;
 }
 
+// f() without the interpreter's lock, which is held again whether f returns or throws.
 template <class F>
 int without_gil(F f) {
-  int rc;
-  Py_BEGIN_ALLOW_THREADS rc = f();
-  Py_END_ALLOW_THREADS return rc;
+  struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+  } released;
+  return f();
 }
 
 at::Tensor bytes_on(const at::Tensor& like, size_t bytes) {
   return at::empty({(int64_t)std::max<size_t>(bytes, 256)}, like.options().dtype(at::kByte));
 }
 
-// relative_forward(address of esa_rel_attn_fwd, of its size query, stream, q, k, v, bias, starts (bytes of int32), q_start,
-// cu_q, cu_k, scale, dropout_p, seed, keep) -> (status, out, out_low or None, lse, the table); keep: out_low is wanted.
-PyObject* relative_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded([&]() -> PyObject* {
-    TORCH_CHECK(n == 15 && PyBytes_Check(args[7]), "relative_forward: arguments");
-    const auto fn = reinterpret_cast<decltype(&esa_rel_attn_fwd)>(PyLong_AsVoidPtr(args[0]));
-    const auto size_of = reinterpret_cast<decltype(&esa_rel_attn_workspace_size)>(PyLong_AsVoidPtr(args[1]));
-    void* stream = PyLong_AsVoidPtr(args[2]);
-    const at::Tensor &q = tensor_of(args[3]), &k = tensor_of(args[4]), &v = tensor_of(args[5]);
-    const at::Tensor table = tensor_of(args[6]).contiguous();
-    const int* starts = reinterpret_cast<const int*>(PyBytes_AS_STRING(args[7]));
-    const int side = (int)(PyBytes_GET_SIZE(args[7]) / sizeof(int)), buckets = (int)table.size(0);
-    const int* q_start = static_cast<const int*>(pointer_of(args[8]));
-    const at::Tensor &cu_q = tensor_of(args[9]), &cu_k = tensor_of(args[10]);
-    const float scale = (float)PyFloat_AsDouble(args[11]), dropout = (float)PyFloat_AsDouble(args[12]);
-    const unsigned long long seed = PyLong_AsUnsignedLongLong(args[13]);
-    const bool keep = PyObject_IsTrue(args[14]) && q.scalar_type() == at::kBFloat16;
-    if (PyErr_Occurred()) return nullptr;
-    TORCH_CHECK(q.size(0) <= INT32_MAX && k.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && cu_q.numel() <= INT32_MAX,
-                "sizes beyond 32 bits");
-    const int batch = (int)cu_q.numel() - 1, tq = (int)q.size(0), tk = (int)k.size(0), heads = (int)q.size(1), hd = (int)q.size(2);
-    const c10::DeviceGuard on(q.device());
-    at::Tensor out, low, lse, ws;
-    size_t bytes = 0;
-    int rc = size_of(batch, tq, tk, heads, hd, code_of(q), buckets, starts, side, 0, &bytes);
-    if (rc == ESA_OK) {
-      out = at::empty(q.sizes(), q.options());
-      if (keep) low = at::empty(q.sizes(), q.options());
-      lse = at::empty({heads, tq}, q.options().dtype(at::kFloat));
-      ws = bytes_on(q, bytes);
-      rc = without_gil([&] {
-        return fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), code_of(table), buckets, starts, side, q_start,
-                  cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), batch, tq, tk, heads, hd, code_of(q), scale, dropout, seed,
-                  out.data_ptr(), keep ? low.data_ptr() : nullptr, lse.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(),
-                  stream);
-      });
-    }
-    return tuple_of({PyLong_FromLong(rc), wrapped(out), wrapped(low), wrapped(lse), wrapped(table)});
-  });
+// A relative attention call besides its tensors.
+struct RelCall {
+  decltype(&esa_rel_attn_fwd) fwd;
+  decltype(&esa_rel_attn_bwd) bwd;
+  decltype(&esa_rel_attn_workspace_size) size;
+  std::string starts;   // int32 values
+  float scale, dropout;
+  unsigned long long seed;
+  const int* first() const { return reinterpret_cast<const int*>(starts.data()); }
+  int side() const { return (int)(starts.size() / sizeof(int)); }
+  // (addresses of forward, backward and size query, starts (bytes of int32), scale, dropout_p, seed)
+  explicit RelCall(PyObject* const* a)
+      : fwd(reinterpret_cast<decltype(fwd)>(PyLong_AsVoidPtr(a[0]))),
+        bwd(reinterpret_cast<decltype(bwd)>(PyLong_AsVoidPtr(a[1]))),
+        size(reinterpret_cast<decltype(size)>(PyLong_AsVoidPtr(a[2]))),
+        starts(PyBytes_AsString(a[3]), PyBytes_Size(a[3])),
+        scale((float)PyFloat_AsDouble(a[4])),
+        dropout((float)PyFloat_AsDouble(a[5])),
+        seed(PyLong_AsUnsignedLongLong(a[6])) {}
+};
+
+struct RelTensors {
+  at::Tensor q, k, v, table, cu_q, cu_k, q_start, out, low, lse;   // q_start, low: or undefined
+};
+
+void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+const void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// out, low (where kept) and lse of t's inputs; the C entry's status.
+int relative_run(const RelCall& c, RelTensors& t, bool keep) {
+  const at::Tensor &q = t.q, &k = t.k;
+  TORCH_CHECK(q.size(0) <= INT32_MAX && k.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX && t.cu_q.numel() <= INT32_MAX,
+              "sizes beyond 32 bits");
+  const int batch = (int)t.cu_q.numel() - 1, tq = (int)q.size(0), tk = (int)k.size(0), heads = (int)q.size(1), hd = (int)q.size(2);
+  const int buckets = (int)t.table.size(0);
+  const c10::DeviceGuard on(q.device());
+  size_t bytes = 0;
+  if (const int rc = c.size(batch, tq, tk, heads, hd, code_of(q), buckets, c.first(), c.side(), 0, &bytes)) return rc;
+  t.out = at::empty(q.sizes(), q.options());
+  if (keep && q.scalar_type() == at::kBFloat16) t.low = at::empty(q.sizes(), q.options());
+  t.lse = at::empty({heads, tq}, q.options().dtype(at::kFloat));
+  const at::Tensor ws = bytes_on(q, bytes);
+  return c.fwd(q.data_ptr(), k.data_ptr(), t.v.data_ptr(), t.table.data_ptr(), code_of(t.table), buckets, c.first(), c.side(),
+               static_cast<const int*>(data_or_null(t.q_start)), t.cu_q.data_ptr<int>(), t.cu_k.data_ptr<int>(), batch, tq, tk,
+               heads, hd, code_of(q), c.scale, c.dropout, c.seed, t.out.data_ptr(), t.low.defined() ? t.low.data_ptr() : nullptr,
+               t.lse.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream_of(q));
 }
 
 // A gradient as the kernels take it: dense, by value, on a 16-byte boundary.
-at::Tensor gradient_of(PyObject* o) {
-  const at::Tensor g = tensor_of(o).resolve_neg().contiguous();
+at::Tensor gradient_of(const at::Tensor& grad) {
+  const at::Tensor g = grad.resolve_neg().contiguous();
   return reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 ? g.clone() : g;
 }
 
-// relative_backward(address of esa_rel_attn_bwd, of its size query, stream, dout, q, k, v, out, out_low, lse, table, starts,
-// q_start, cu_q, cu_k, scale, dropout_p, seed) -> (status, dq, dk, dv, dtable in the table's type); arguments as the
-// forward's and its results
+// d: dq, dk, dv and the table's gradient in the table's type; the C entry's status.
+int relative_back(const RelCall& c, const RelTensors& t, const at::Tensor& grad, at::Tensor (&d)[4]) {
+  const at::Tensor &q = t.q, &k = t.k;
+  const int batch = (int)t.cu_q.numel() - 1, tq = (int)q.size(0), tk = (int)k.size(0), heads = (int)q.size(1), hd = (int)q.size(2);
+  const int buckets = (int)t.table.size(0);
+  const c10::DeviceGuard on(q.device());
+  const at::Tensor g = gradient_of(grad);
+  size_t bytes = 0;
+  int rc = c.size(batch, tq, tk, heads, hd, code_of(q), buckets, c.first(), c.side(), 1, &bytes);
+  if (rc) return rc;
+  d[0] = at::empty(q.sizes(), q.options());
+  d[1] = at::empty(k.sizes(), k.options());
+  d[2] = at::empty(k.sizes(), k.options());
+  d[3] = at::empty(t.table.sizes(), t.table.options().dtype(at::kFloat));
+  const at::Tensor ws = bytes_on(q, bytes);
+  rc = c.bwd(g.data_ptr(), q.data_ptr(), k.data_ptr(), t.v.data_ptr(), t.out.data_ptr(), data_or_null(t.low),
+             t.lse.data_ptr<float>(), t.table.data_ptr(), code_of(t.table), buckets, c.first(), c.side(),
+             static_cast<const int*>(data_or_null(t.q_start)), t.cu_q.data_ptr<int>(), t.cu_k.data_ptr<int>(), batch, tq, tk, heads,
+             hd, code_of(q), c.scale, c.dropout, c.seed, d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), d[3].data_ptr<float>(),
+             ws.data_ptr(), (size_t)ws.numel(), stream_of(q));
+  if (rc == ESA_OK && t.table.scalar_type() != at::kFloat) d[3] = d[3].to(t.table.scalar_type());
+  return rc;
+}
+
+at::Tensor optional(PyObject* o) { return o == Py_None ? at::Tensor() : tensor_of(o); }
+
+// (q, k, v, bias, q_start, cu_q, cu_k)
+RelTensors relative_inputs(PyObject* const* a) {
+  RelTensors t;
+  t.q = tensor_of(a[0]);
+  t.k = tensor_of(a[1]);
+  t.v = tensor_of(a[2]);
+  t.table = tensor_of(a[3]).contiguous();
+  t.q_start = optional(a[4]);
+  t.cu_q = tensor_of(a[5]);
+  t.cu_k = tensor_of(a[6]);
+  return t;
+}
+
+// relative_forward(RelCall's seven, relative_inputs' seven, keep) -> (status, out, out_low or None, lse, the table)
+PyObject* relative_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 15 && PyBytes_Check(args[3]), "relative_forward: arguments");
+    const RelCall c(args);
+    RelTensors t = relative_inputs(args + 7);
+    const bool keep = PyObject_IsTrue(args[14]);
+    if (PyErr_Occurred()) return nullptr;
+    const int rc = without_gil([&] { return relative_run(c, t, keep); });
+    return tuple_of({PyLong_FromLong(rc), wrapped(t.out), wrapped(t.low), wrapped(t.lse), wrapped(t.table)});
+  });
+}
+
+// relative_backward(RelCall's seven, relative_inputs' seven, out, out_low, lse, dout) -> (status, dq, dk, dv, dtable)
 PyObject* relative_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    TORCH_CHECK(n == 18 && PyBytes_Check(args[11]), "relative_backward: arguments");
-    const auto fn = reinterpret_cast<decltype(&esa_rel_attn_bwd)>(PyLong_AsVoidPtr(args[0]));
-    const auto size_of = reinterpret_cast<decltype(&esa_rel_attn_workspace_size)>(PyLong_AsVoidPtr(args[1]));
-    void* stream = PyLong_AsVoidPtr(args[2]);
-    const at::Tensor &q = tensor_of(args[4]), &k = tensor_of(args[5]), &v = tensor_of(args[6]), &out = tensor_of(args[7]);
-    const void* low = pointer_of(args[8]);
-    const at::Tensor &lse = tensor_of(args[9]), &table = tensor_of(args[10]);
-    const int* starts = reinterpret_cast<const int*>(PyBytes_AS_STRING(args[11]));
-    const int side = (int)(PyBytes_GET_SIZE(args[11]) / sizeof(int)), buckets = (int)table.size(0);
-    const int* q_start = static_cast<const int*>(pointer_of(args[12]));
-    const at::Tensor &cu_q = tensor_of(args[13]), &cu_k = tensor_of(args[14]);
-    const float scale = (float)PyFloat_AsDouble(args[15]), dropout = (float)PyFloat_AsDouble(args[16]);
-    const unsigned long long seed = PyLong_AsUnsignedLongLong(args[17]);
+    TORCH_CHECK(n == 18 && PyBytes_Check(args[3]), "relative_backward: arguments");
+    const RelCall c(args);
+    RelTensors t = relative_inputs(args + 7);
+    t.out = tensor_of(args[14]);
+    t.low = optional(args[15]);
+    t.lse = tensor_of(args[16]);
+    const at::Tensor& g = tensor_of(args[17]);
     if (PyErr_Occurred()) return nullptr;
-    const int batch = (int)cu_q.numel() - 1, tq = (int)q.size(0), tk = (int)k.size(0), heads = (int)q.size(1), hd = (int)q.size(2);
-    const c10::DeviceGuard on(q.device());
-    const at::Tensor g = gradient_of(args[3]);
-    at::Tensor dq, dk, dv, dtable;
-    size_t bytes = 0;
-    int rc = size_of(batch, tq, tk, heads, hd, code_of(q), buckets, starts, side, 1, &bytes);
-    if (rc == ESA_OK) {
-      dq = at::empty(q.sizes(), q.options());
-      dk = at::empty(k.sizes(), k.options());
-      dv = at::empty(v.sizes(), v.options());
-      dtable = at::empty(table.sizes(), table.options().dtype(at::kFloat));
-      const at::Tensor ws = bytes_on(q, bytes);
-      rc = without_gil([&] {
-        return fn(g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low, lse.data_ptr<float>(),
-                  table.data_ptr(), code_of(table), buckets, starts, side, q_start, cu_q.data_ptr<int>(), cu_k.data_ptr<int>(),
-                  batch, tq, tk, heads, hd, code_of(q), scale, dropout, seed, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                  dtable.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream);
-      });
-      if (rc == ESA_OK && table.scalar_type() != at::kFloat) dtable = dtable.to(table.scalar_type());
+    at::Tensor d[4];
+    const int rc = without_gil([&] { return relative_back(c, t, g, d); });
+    return tuple_of({PyLong_FromLong(rc), wrapped(d[0]), wrapped(d[1]), wrapped(d[2]), wrapped(d[3])});
+  });
+}
+
+// ---- the same as autograd nodes, for ordinary eager calls
+
+// Results of a backward that is itself recorded: differentiating them again is refused.
+torch::autograd::variable_list only_once(torch::autograd::variable_list&& grads, bool recorded) {
+  if (!recorded) return std::move(grads);
+  for (at::Tensor& g : grads)
+    if (g.defined()) {
+      g = g.detach();
+      g.requires_grad_(true);
     }
-    return tuple_of({PyLong_FromLong(rc), wrapped(dq), wrapped(dk), wrapped(dv), wrapped(dtable)});
+  const auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      "these gradients cannot be differentiated again", (int64_t)grads.size());
+  return (*refuse)(std::move(grads));
+}
+
+using torch::autograd::SavedVariable;
+
+struct RelativeAttentionBackward : torch::autograd::Node {
+  RelCall call;
+  SavedVariable q, k, v, table, cu_q, cu_k, q_start, out, low, lse;
+  std::mutex mutex;
+  explicit RelativeAttentionBackward(const RelCall& c) : call(c) {}
+  std::string name() const override { return "RelativeAttentionBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex);
+    for (SavedVariable* x : {&q, &k, &v, &table, &cu_q, &cu_k, &q_start, &out, &low, &lse}) x->reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex);
+    torch::autograd::variable_list result(4);
+    if (!grads[0].defined()) return result;
+    const bool recorded = at::GradMode::is_enabled();
+    const at::AutoGradMode none(false);
+    RelTensors t;
+    t.q = q.unpack();
+    t.k = k.unpack();
+    t.v = v.unpack();
+    t.table = table.unpack();
+    t.cu_q = cu_q.unpack();
+    t.cu_k = cu_k.unpack();
+    t.q_start = q_start.unpack();
+    t.out = out.unpack(getptr());
+    t.low = low.unpack();
+    t.lse = lse.unpack();
+    at::Tensor d[4];
+    const int rc = relative_back(call, t, grads[0], d);
+    TORCH_CHECK(rc == ESA_OK, "esa_rel_attn_bwd: status ", rc);
+    for (int i = 0; i < 4; ++i) result[i] = d[i];
+    return only_once(std::move(result), recorded);
+  }
+};
+
+bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// relative(RelCall's seven, relative_inputs' seven) -> (status, out, lse), recorded where torch would
+PyObject* relative(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 14 && PyBytes_Check(args[3]), "relative: arguments");
+    const RelCall c(args);
+    RelTensors t = relative_inputs(args + 7);
+    const at::Tensor& bias = tensor_of(args[10]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool record = at::GradMode::is_enabled() && (wants_grad(t.q) || wants_grad(t.k) || wants_grad(t.v) || wants_grad(bias));
+    int rc;
+    {
+      const at::AutoGradMode none(false);
+      if (record) t.table = t.table.detach();
+      rc = without_gil([&] { return relative_run(c, t, record); });
+    }
+    if (rc == ESA_OK && record) {
+      std::shared_ptr<RelativeAttentionBackward> node(new RelativeAttentionBackward(c), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(t.q, t.k, t.v, bias));
+      torch::autograd::set_history(t.out, node);
+      node->q = SavedVariable(t.q, false);
+      node->k = SavedVariable(t.k, false);
+      node->v = SavedVariable(t.v, false);
+      // the bias itself where it was read as it lies, for the check that it has not been written since
+      node->table = SavedVariable(bias.is_contiguous() ? bias : t.table, false);
+      node->cu_q = SavedVariable(t.cu_q, false);
+      node->cu_k = SavedVariable(t.cu_k, false);
+      node->q_start = SavedVariable(t.q_start, false);
+      node->out = SavedVariable(t.out, true);
+      node->low = SavedVariable(t.low, false);
+      node->lse = SavedVariable(t.lse, false);
+    }
+    return tuple_of({PyLong_FromLong(rc), wrapped(t.out), wrapped(t.lse)});
   });
 }
 
@@ -469,98 +611,199 @@ at::Tensor rows_of(const at::Tensor& x) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
-// qk_norm_forward(address of esa_qk_norm_fwd, stream, q, k, wq, wk (float32), positions, frequencies, eps, interleaved) ->
-// (status, q_out, k_out or None, q's rows, k's rows or None)
+// A call of the norms with rotation besides its tensors.
+struct NormCall {
+  decltype(&esa_qk_norm_fwd) fwd;
+  decltype(&esa_qk_norm_bwd) bwd;
+  decltype(&esa_qk_norm_bwd_workspace_size) size;
+  float eps;
+  int interleaved;
+  // (addresses of forward, backward and the backward's size query, eps, interleaved)
+  explicit NormCall(PyObject* const* a)
+      : fwd(reinterpret_cast<decltype(fwd)>(PyLong_AsVoidPtr(a[0]))),
+        bwd(reinterpret_cast<decltype(bwd)>(PyLong_AsVoidPtr(a[1]))),
+        size(reinterpret_cast<decltype(size)>(PyLong_AsVoidPtr(a[2]))),
+        eps((float)PyFloat_AsDouble(a[3])),
+        interleaved(PyObject_IsTrue(a[4])) {}
+};
+
+struct NormTensors {
+  at::Tensor q, k, wq, wk, positions, frequencies;   // rows where they are read; weights in float32; all but q may be undefined
+  bool keys() const { return k.defined(); }
+  int heads_k() const { return keys() ? (int)k.size(1) : 0; }
+  int rotary() const { return frequencies.defined() ? 2 * (int)frequencies.numel() : 0; }
+  int positions_bytes() const { return positions.defined() ? (int)positions.element_size() : 0; }
+  const float* weight(const at::Tensor& w) const { return static_cast<const float*>(data_or_null(w)); }
+  void strides(long long (&x)[4]) const {
+    x[0] = q.stride(0);
+    x[1] = q.stride(1);
+    x[2] = keys() ? k.stride(0) : 0;
+    x[3] = keys() ? k.stride(1) : 0;
+  }
+};
+
+at::Tensor f32_of(const at::Tensor& w) { return w.defined() ? w.detach().to(at::kFloat).contiguous() : w; }
+
+// (q, k, q_weight, k_weight, positions, frequencies)
+NormTensors norm_inputs(PyObject* const* a) {
+  NormTensors t;
+  t.q = rows_of(tensor_of(a[0]));
+  if (a[1] != Py_None) t.k = rows_of(tensor_of(a[1]));
+  t.wq = f32_of(optional(a[2]));
+  t.wk = f32_of(optional(a[3]));
+  t.positions = optional(a[4]);
+  t.frequencies = optional(a[5]);
+  return t;
+}
+
+int norm_run(const NormCall& c, const NormTensors& t, at::Tensor& q_out, at::Tensor& k_out) {
+  TORCH_CHECK(t.q.size(0) <= INT32_MAX, "sizes beyond 32 bits");
+  long long strides[4];
+  t.strides(strides);
+  const c10::DeviceGuard on(t.q.device());
+  q_out = at::empty(t.q.sizes(), t.q.options());
+  if (t.keys()) k_out = at::empty(t.k.sizes(), t.k.options());
+  return c.fwd(t.q.data_ptr(), data_or_null(t.k), strides, (int)t.q.size(0), (int)t.q.size(1), t.heads_k(), (int)t.q.size(2),
+               code_of(t.q), t.weight(t.wq), t.weight(t.wk), data_or_null(t.positions), t.positions_bytes(),
+               static_cast<const double*>(data_or_null(t.frequencies)), t.rotary(), c.interleaved, c.eps, q_out.data_ptr(),
+               k_out.defined() ? k_out.data_ptr() : nullptr, stream_of(t.q));
+}
+
+// d: dq, dk and where their types (c10::ScalarType) are given, the weights' gradients.
+int norm_back(const NormCall& c, const NormTensors& t, const at::Tensor& grad_q, const at::Tensor& grad_k,
+              const std::optional<at::ScalarType> (&types)[2], at::Tensor (&d)[4]) {
+  long long strides[4];
+  t.strides(strides);
+  const int total = (int)t.q.size(0), hd = (int)t.q.size(2);
+  const c10::DeviceGuard on(t.q.device());
+  auto given = [](const at::Tensor& g, const at::Tensor& like) {
+    return gradient_of(g.defined() ? g : at::zeros(like.sizes(), like.options()));
+  };
+  const at::Tensor gq = given(grad_q, t.q), gk = t.keys() ? given(grad_k, t.k) : at::Tensor();
+  d[0] = at::empty(t.q.sizes(), t.q.options());
+  if (t.keys()) d[1] = at::empty(t.k.sizes(), t.k.options());
+  at::Tensor ws;
+  for (int i = 0; i < 2; ++i)
+    if (types[i]) d[2 + i] = at::empty({hd}, t.q.options().dtype(at::kFloat));
+  if (types[0] || types[1]) {
+    size_t bytes = 0;
+    if (const int rc = c.size(total, hd, &bytes)) return rc;
+    ws = bytes_on(t.q, bytes);
+  }
+  auto floats = [](const at::Tensor& x) { return x.defined() ? x.data_ptr<float>() : nullptr; };
+  const int rc = c.bwd(gq.data_ptr(), data_or_null(gk), t.q.data_ptr(), data_or_null(t.k), strides, total, (int)t.q.size(1),
+                       t.heads_k(), hd, code_of(t.q), t.weight(t.wq), t.weight(t.wk), data_or_null(t.positions),
+                       t.positions_bytes(), static_cast<const double*>(data_or_null(t.frequencies)), t.rotary(), c.interleaved,
+                       c.eps, d[0].data_ptr(), t.keys() ? d[1].data_ptr() : nullptr, floats(d[2]), floats(d[3]),
+                       ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream_of(t.q));
+  for (int i = 0; i < 2; ++i)
+    if (rc == ESA_OK && types[i]) d[2 + i] = d[2 + i].to(*types[i]);
+  return rc;
+}
+
+// qk_norm_forward(NormCall's five, norm_inputs' six) -> (status, q_out, k_out or None, q's rows, k's rows or None)
 PyObject* qk_norm_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    TORCH_CHECK(n == 10, "qk_norm_forward: arguments");
-    const auto fn = reinterpret_cast<decltype(&esa_qk_norm_fwd)>(PyLong_AsVoidPtr(args[0]));
-    void* stream = PyLong_AsVoidPtr(args[1]);
-    const at::Tensor q = rows_of(tensor_of(args[2]));
-    at::Tensor k;
-    if (args[3] != Py_None) k = rows_of(tensor_of(args[3]));
-    const float *wq = static_cast<const float*>(pointer_of(args[4])), *wk = static_cast<const float*>(pointer_of(args[5]));
-    const void* positions = pointer_of(args[6]);
-    const int positions_bytes = positions || args[6] != Py_None ? (int)tensor_of(args[6]).element_size() : 0;
-    const double* frequencies = static_cast<const double*>(pointer_of(args[7]));
-    const int rotary = args[7] != Py_None ? 2 * (int)tensor_of(args[7]).numel() : 0;
-    const float eps = (float)PyFloat_AsDouble(args[8]);
-    const int interleaved = PyObject_IsTrue(args[9]);
+    TORCH_CHECK(n == 11, "qk_norm_forward: arguments");
+    const NormCall c(args);
+    const NormTensors t = norm_inputs(args + 5);
     if (PyErr_Occurred()) return nullptr;
-    TORCH_CHECK(q.size(0) <= INT32_MAX, "sizes beyond 32 bits");
-    const long long strides[4] = {q.stride(0), q.stride(1), k.defined() ? k.stride(0) : 0, k.defined() ? k.stride(1) : 0};
-    const c10::DeviceGuard on(q.device());
-    const at::Tensor q_out = at::empty(q.sizes(), q.options());
-    at::Tensor k_out;
-    if (k.defined()) k_out = at::empty(k.sizes(), k.options());
-    const int rc = without_gil([&] {
-      return fn(q.data_ptr(), k.defined() ? k.data_ptr() : nullptr, strides, (int)q.size(0), (int)q.size(1),
-                k.defined() ? (int)k.size(1) : 0, (int)q.size(2), code_of(q), wq, wk, positions, positions_bytes, frequencies,
-                rotary, interleaved, eps, q_out.data_ptr(), k_out.defined() ? k_out.data_ptr() : nullptr, stream);
-    });
-    return tuple_of({PyLong_FromLong(rc), wrapped(q_out), wrapped(k_out), wrapped(q), wrapped(k)});
+    at::Tensor q_out, k_out;
+    const int rc = without_gil([&] { return norm_run(c, t, q_out, k_out); });
+    return tuple_of({PyLong_FromLong(rc), wrapped(q_out), wrapped(k_out), wrapped(t.q), wrapped(t.k)});
   });
 }
 
-// qk_norm_backward(address of esa_qk_norm_bwd, of its size query, stream, gq, gk, q, k, wq, wk, positions, frequencies, eps,
-// interleaved, type code of dwq or None, of dwk) -> (status, dq, dk or None, dwq or None, dwk or None); q and k the rows
-// that the forward returned; type codes: ESA_F32, ESA_BF16
+// qk_norm_backward(NormCall's five, norm_inputs' six (the forward's rows; the weights themselves), gq, gk or None, whether
+// the weights' gradients are wanted) -> (status, dq, dk or None, dwq or None, dwk or None)
 PyObject* qk_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     TORCH_CHECK(n == 15, "qk_norm_backward: arguments");
-    const auto fn = reinterpret_cast<decltype(&esa_qk_norm_bwd)>(PyLong_AsVoidPtr(args[0]));
-    const auto size_of = reinterpret_cast<decltype(&esa_qk_norm_bwd_workspace_size)>(PyLong_AsVoidPtr(args[1]));
-    void* stream = PyLong_AsVoidPtr(args[2]);
-    const at::Tensor& q = tensor_of(args[5]);
-    const bool keys = args[6] != Py_None;
-    const at::Tensor& k = keys ? tensor_of(args[6]) : q;
-    const float *wq = static_cast<const float*>(pointer_of(args[7])), *wk = static_cast<const float*>(pointer_of(args[8]));
-    const void* positions = pointer_of(args[9]);
-    const int positions_bytes = args[9] != Py_None ? (int)tensor_of(args[9]).element_size() : 0;
-    const double* frequencies = static_cast<const double*>(pointer_of(args[10]));
-    const int rotary = args[10] != Py_None ? 2 * (int)tensor_of(args[10]).numel() : 0;
-    const float eps = (float)PyFloat_AsDouble(args[11]);
-    const int interleaved = PyObject_IsTrue(args[12]);
-    const long code[2] = {args[13] == Py_None ? -1 : PyLong_AsLong(args[13]), args[14] == Py_None ? -1 : PyLong_AsLong(args[14])};
+    const NormCall c(args);
+    const NormTensors t = norm_inputs(args + 5);
+    const at::Tensor gq = optional(args[11]), gk = optional(args[12]);
+    std::optional<at::ScalarType> types[2];
+    for (int i = 0; i < 2; ++i)
+      if (args[7 + i] != Py_None && PyObject_IsTrue(args[13 + i])) types[i] = tensor_of(args[7 + i]).scalar_type();
     if (PyErr_Occurred()) return nullptr;
-    const long long strides[4] = {q.stride(0), q.stride(1), keys ? k.stride(0) : 0, keys ? k.stride(1) : 0};
-    const int total = (int)q.size(0), hd = (int)q.size(2);
-    const c10::DeviceGuard on(q.device());
-    const at::Tensor gq = gradient_of(args[3]), dq = at::empty(q.sizes(), q.options());
-    at::Tensor gk, dk, dw[2], ws;
-    if (keys) {
-      gk = gradient_of(args[4]);
-      dk = at::empty(k.sizes(), k.options());
+    at::Tensor d[4];
+    const int rc = without_gil([&] { return norm_back(c, t, gq, gk, types, d); });
+    return tuple_of({PyLong_FromLong(rc), wrapped(d[0]), wrapped(d[1]), wrapped(d[2]), wrapped(d[3])});
+  });
+}
+
+struct QkNormBackward : torch::autograd::Node {
+  NormCall call;
+  std::optional<at::ScalarType> types[2];
+  SavedVariable q, k, wq, wk, positions, frequencies;
+  std::mutex mutex;
+  explicit QkNormBackward(const NormCall& c) : call(c) {}
+  std::string name() const override { return "QkNormBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex);
+    for (SavedVariable* x : {&q, &k, &wq, &wk, &positions, &frequencies}) x->reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex);
+    const bool recorded = at::GradMode::is_enabled();
+    const at::AutoGradMode none(false);
+    NormTensors t;
+    t.q = q.unpack();
+    t.k = k.unpack();
+    t.wq = f32_of(wq.unpack());
+    t.wk = f32_of(wk.unpack());
+    t.positions = positions.unpack();
+    t.frequencies = frequencies.unpack();
+    at::Tensor d[4];
+    const int rc = norm_back(call, t, grads[0], grads.size() > 1 ? grads[1] : at::Tensor(), types, d);
+    TORCH_CHECK(rc == ESA_OK, "esa_qk_norm_bwd: status ", rc);
+    return only_once({d[0], d[1], d[2], d[3]}, recorded);
+  }
+};
+
+// qk_norm(NormCall's five, norm_inputs' six) -> (status, q_out, k_out or None), recorded where torch would
+PyObject* qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 11, "qk_norm: arguments");
+    const NormCall c(args);
+    const at::Tensor q = tensor_of(args[5]), k = optional(args[6]), wq = optional(args[7]), wk = optional(args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool record = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(wq) || wants_grad(wk));
+    at::Tensor q_out, k_out;
+    NormTensors t;
+    int rc;
+    {
+      const at::AutoGradMode none(false);
+      t = norm_inputs(args + 5);
+      rc = without_gil([&] { return norm_run(c, t, q_out, k_out); });
     }
-    int rc = ESA_OK;
-    for (int i = 0; i < 2; ++i)
-      if (code[i] >= 0) dw[i] = at::empty({hd}, q.options().dtype(at::kFloat));
-    if (dw[0].defined() || dw[1].defined()) {
-      size_t bytes = 0;
-      rc = size_of(total, hd, &bytes);
-      if (rc == ESA_OK) ws = bytes_on(q, bytes);
+    if (rc == ESA_OK && record) {
+      std::shared_ptr<QkNormBackward> node(new QkNormBackward(c), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(q, k, wq, wk));
+      if (wants_grad(wq)) node->types[0] = wq.scalar_type();
+      if (wants_grad(wk)) node->types[1] = wk.scalar_type();
+      torch::autograd::set_history(q_out, node);
+      if (k_out.defined()) torch::autograd::set_history(k_out, node);
+      node->q = SavedVariable(t.q, false);
+      node->k = SavedVariable(t.k, false);
+      node->wq = SavedVariable(wq, false);
+      node->wk = SavedVariable(wk, false);
+      node->positions = SavedVariable(t.positions, false);
+      node->frequencies = SavedVariable(t.frequencies, false);
     }
-    if (rc == ESA_OK)
-      rc = without_gil([&] {
-        return fn(gq.data_ptr(), keys ? gk.data_ptr() : nullptr, q.data_ptr(), keys ? k.data_ptr() : nullptr, strides, total,
-                  (int)q.size(1), keys ? (int)k.size(1) : 0, hd, code_of(q), wq, wk, positions, positions_bytes, frequencies,
-                  rotary, interleaved, eps, dq.data_ptr(), keys ? dk.data_ptr() : nullptr,
-                  dw[0].defined() ? dw[0].data_ptr<float>() : nullptr, dw[1].defined() ? dw[1].data_ptr<float>() : nullptr,
-                  ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream);
-      });
-    for (int i = 0; i < 2; ++i)
-      if (rc == ESA_OK && code[i] == kBf16) dw[i] = dw[i].to(at::kBFloat16);
-    return tuple_of({PyLong_FromLong(rc), wrapped(dq), wrapped(dk), wrapped(dw[0]), wrapped(dw[1])});
+    return tuple_of({PyLong_FromLong(rc), wrapped(q_out), wrapped(k_out)});
   });
 }
 
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)); }
 
 PyMethodDef methods[] = {{"relative_fits", fast(relative_fits), METH_FASTCALL, nullptr},
+                         {"relative", fast(relative), METH_FASTCALL, nullptr},
                          {"relative_forward", fast(relative_forward), METH_FASTCALL, nullptr},
                          {"relative_backward", fast(relative_backward), METH_FASTCALL, nullptr},
                          {"qk_norm_backward", fast(qk_norm_backward), METH_FASTCALL, nullptr},
                          {"qk_norm_fits", fast(qk_norm_fits), METH_FASTCALL, nullptr},
+                         {"qk_norm", fast(qk_norm), METH_FASTCALL, nullptr},
                          {"qk_norm_forward", fast(qk_norm_forward), METH_FASTCALL, nullptr},
                          {"clip", fast(clip), METH_FASTCALL, nullptr},
                          {"describe", describe, METH_O, nullptr},

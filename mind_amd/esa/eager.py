@@ -60,11 +60,4 @@ def call(function, *args):
     return function.apply(*args)
 
 
-FITS, EXACT, GRAD = 1, 2, 4   # what the host module's checks say of a call (csrc/esa_tensors.cpp)
-
-
-def call_checked(flags: int, function, *args):
-    """``call`` where the host module has looked at the tensors."""
-    if flags & EXACT and not (flags & GRAD and torch.is_grad_enabled()) and ordinary():
-        return function.forward(Unrecorded(), *args)
-    return function.apply(*args)
+FITS, EXACT = 1, 2   # what the host module's checks say of a call (csrc/esa_tensors.cpp)

@@ -14,8 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .attention import HEAD_DIMS
-from .eager import FITS, call_checked
-from .layer_norm import f32_values
+from .eager import EXACT, FITS, ordinary
 
 _CODES = {torch.float32: _lib.ESA_F32, torch.bfloat16: _lib.ESA_BF16}
 MAX_HEADS = 2048
@@ -28,29 +27,30 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, device=None) -> t
     return float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
 
 
+def _call(eps, interleaved):
+    """What the host module takes of a call besides its tensors."""
+    return (_lib.address("esa_qk_norm_fwd"), _lib.address("esa_qk_norm_bwd"), _lib.address("esa_qk_norm_bwd_workspace_size"),
+            eps, interleaved)
+
+
 class _QkNorm(torch.autograd.Function):
+    """The call where torch has to see it as a function (under transforms, tracing and dispatch modes, over subclasses);
+    ordinary eager calls are a node of the host module's."""
+
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
-        ctx.weight_dtypes = [None if w is None else w.dtype for w in (q_weight, k_weight)]
-        wq, wk = f32_values(q_weight), f32_values(k_weight)
-        rc, q_out, k_out, q, k = _lib.tensors().qk_norm_forward(_lib.address("esa_qk_norm_fwd"), _lib.stream_of(q), q, k, wq, wk,
-                                                                positions, frequencies, eps, interleaved)
+        ctx.call = _call(eps, interleaved)
+        rc, q_out, k_out, q, k = _lib.tensors().qk_norm_forward(*ctx.call, q, k, q_weight, k_weight, positions, frequencies)
         _lib.check(rc, "esa_qk_norm_fwd")
-        ctx.save_for_backward(q, k, wq, wk, positions, frequencies)
-        ctx.meta = (eps, interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk=None):
-        q, k, wq, wk, positions, frequencies = ctx.saved_tensors
-        eps, interleaved = ctx.meta
-        wanted = [_CODES[t] if n else None for n, t in zip(ctx.needs_input_grad[2:4], ctx.weight_dtypes)]
-        rc, dq, dk, dwq, dwk = _lib.tensors().qk_norm_backward(
-            _lib.address("esa_qk_norm_bwd"), _lib.address("esa_qk_norm_bwd_workspace_size"), _lib.stream_of(q), gq, gk, q, k, wq, wk,
-            positions, frequencies, eps, interleaved, *wanted)
+        rc, *grads = _lib.tensors().qk_norm_backward(*ctx.call, *ctx.saved_tensors, gq, gk, *ctx.needs_input_grad[2:4])
         _lib.check(rc, "esa_qk_norm_bwd")
-        return dq, dk, dwq, dwk, None, None, None, None
+        return *grads, None, None, None, None
 
 
 def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor | None = None) -> None:
@@ -112,4 +112,8 @@ def qk_norm_rotary(q, k=None, q_weight=None, k_weight=None, positions=None, freq
         _lib.require_on_one_gpu(q, k, q_weight, k_weight, positions, frequencies)
         q, k, q_weight, k_weight, frequencies = (None if t is None else t.resolve_neg()
                                                  for t in (q, k, q_weight, k_weight, frequencies))
-    return call_checked(flags, _QkNorm, q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))
+    if flags & EXACT and ordinary():
+        rc, q_out, k_out = _lib.tensors().qk_norm(*_call(eps, bool(interleaved)), q, k, q_weight, k_weight, positions, frequencies)
+        _lib.check(rc, "esa_qk_norm_fwd")
+        return q_out if k is None else (q_out, k_out)
+    return _QkNorm.apply(q, k, q_weight, k_weight, positions, frequencies, eps, bool(interleaved))

@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .attention import _SEED_MASK, _check_dropout, _check_index, _check_tokens, draw_dropout_seed
-from .eager import FITS, call_checked
+from .eager import EXACT, FITS, ordinary
 
 MAX_REACH, MAX_BUCKETS = 768, 256
 _TABLE = (torch.float32, torch.bfloat16)
@@ -59,18 +59,27 @@ def _start_bytes(starts: tuple[int, ...]) -> bytes:
     return bytes((ctypes.c_int * len(starts))(*starts))
 
 
+def _call(starts, scale, dropout_p, seed):
+    """What the host module takes of a call besides its tensors."""
+    return (_lib.address("esa_rel_attn_fwd"), _lib.address("esa_rel_attn_bwd"), _lib.address("esa_rel_attn_workspace_size"),
+            _start_bytes(starts), scale, dropout_p, seed)
+
+
 class _RelativeAttention(torch.autograd.Function):
+    """The call where torch has to see it as a function (under transforms, tracing and dispatch modes, over subclasses);
+    ordinary eager calls are a node of the host module's."""
+
     @staticmethod
     def forward(ctx, q, k, v, bias, cu_q, cu_k, q_start, starts, scale, dropout_p, seed):
         # kept for a backward: what the rounding of a bf16 out leaves, so that its row statistic has none
-        rc, out, low, lse, table = _lib.tensors().relative_forward(
-            _lib.address("esa_rel_attn_fwd"), _lib.address("esa_rel_attn_workspace_size"), _lib.stream_of(q), q, k, v, bias,
-            _start_bytes(starts), q_start, cu_q, cu_k, scale, dropout_p, seed, any(ctx.needs_input_grad))
+        call = _call(starts, scale, dropout_p, seed)
+        rc, out, low, lse, table = _lib.tensors().relative_forward(*call, q, k, v, bias, q_start, cu_q, cu_k,
+                                                                   any(ctx.needs_input_grad))
         _lib.check(rc, "esa_rel_attn_fwd")
         ctx.save_for_backward(q, k, v, table, out, low, lse, cu_q, cu_k, q_start)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(lse)
-        ctx.meta = (starts, scale, dropout_p, seed)
+        ctx.call = call
         return out, lse
 
     @staticmethod
@@ -79,10 +88,7 @@ class _RelativeAttention(torch.autograd.Function):
         q, k, v, table, out, low, lse, cu_q, cu_k, q_start = ctx.saved_tensors
         if g is None:
             return (None,) * 11
-        starts, scale, dropout_p, seed = ctx.meta
-        rc, dq, dk, dv, dtable = _lib.tensors().relative_backward(
-            _lib.address("esa_rel_attn_bwd"), _lib.address("esa_rel_attn_workspace_size"), _lib.stream_of(q), g, q, k, v, out, low,
-            lse, table, _start_bytes(starts), q_start, cu_q, cu_k, scale, dropout_p, seed)
+        rc, dq, dk, dv, dtable = _lib.tensors().relative_backward(*ctx.call, q, k, v, table, q_start, cu_q, cu_k, out, low, lse, g)
         _lib.check(rc, "esa_rel_attn_bwd")
         return dq, dk, dv, dtable, None, None, None, None, None, None, None
 
@@ -137,6 +143,11 @@ def relative_attention(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=N
     if not flags & FITS:
         _lib.require_on_one_gpu(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start)
         q, k, v, bias = (t.resolve_neg() for t in (q, k, v, bias))
-    out, lse = call_checked(flags, _RelativeAttention, q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start, starts, scale,
-                            dropout_p, int(dropout_seed or 0) & _SEED_MASK)
+    seed = int(dropout_seed or 0) & _SEED_MASK
+    if flags & EXACT and ordinary():
+        rc, out, lse = _lib.tensors().relative(*_call(starts, scale, dropout_p, seed), q, k, v, bias, q_start, cu_seqlens_q,
+                                               cu_seqlens_k)
+        _lib.check(rc, "esa_rel_attn_fwd")
+    else:
+        out, lse = _RelativeAttention.apply(q, k, v, bias, cu_seqlens_q, cu_seqlens_k, q_start, starts, scale, dropout_p, seed)
     return (out, lse) if return_lse else out

@@ -11,17 +11,21 @@ backward, added as independent errors sqrt(64) 2^-9 = 1.6e-2 of a norm; held to 
 """
 import copy
 import math
+import threading
 
 import numpy as np
 import pytest
 import torch
 from torch.nn import functional as F
+from torch.utils.checkpoint import checkpoint
 
 from mind_amd import generators
 from mind_amd.esa import masked_layers as ML
 from mind_amd.esa.gradients import clip_grad_norm_
 from mind_amd.esa.graphs import GraphedForward
 from mind_amd.esa.packing import EdgeAdjacency
+from mind_amd.esa.qk_norm import qk_norm_rotary, rotary_frequencies
+from mind_amd.esa.relative import relative_attention
 from mind_amd.esa.token_order import TokenOrder
 from tests.test_gpu_relative import buckets_of
 
@@ -218,3 +222,91 @@ def test_without_an_order_nothing_changes(device):
     with torch.no_grad():
         e, r = flat.forward_packed(z, one)[1], flat.forward_packed(z.flip(0).contiguous(), one)[1].flip(0)
     assert float((e - r).norm() / e.norm()) > 1e-3
+
+
+def _both(device, dtype=torch.float32):
+    """A chain of both operators: (leaves, function of them)."""
+    gen = torch.Generator(device).manual_seed(11)
+    q, k, v = (torch.randn(120, 3, 16, device=device, dtype=dtype, generator=gen) for _ in range(3))
+    w, bias = torch.rand(16, device=device, generator=gen) + 0.5, torch.randn(8, 3, device=device, generator=gen)
+    cu = torch.tensor([0, 50, 120], dtype=torch.int32, device=device)
+    at, f = torch.arange(120, device=device), rotary_frequencies(8, device=device)
+    leaves = [x.requires_grad_(True) for x in (q, k, v, w, bias)]
+
+    def run(q, k, v, w, bias):
+        a, b = qk_norm_rotary(q, k, w, w, positions=at, frequencies=f)
+        return relative_attention(a, b, v, bias, cu, cu, max_distance=20)
+    return leaves, run
+
+
+def test_as_any_recorded_operation(device):
+    """Graphs kept and used again, checkpoints, saved tensors on the host, leaves without gradients, outputs left out."""
+    leaves, run = _both(device)
+    out = run(*leaves)
+    g = torch.randn_like(out)
+    want = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    same = lambda got: all(torch.equal(x, y) for x, y in zip(got, want))
+    assert same(torch.autograd.grad(out, leaves, g))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, g)   # the graph is gone
+    assert same(torch.autograd.grad(checkpoint(run, *leaves, use_reentrant=False), leaves, g))
+    with torch.autograd.graph.save_on_cpu():
+        out = run(*leaves)
+    assert same(torch.autograd.grad(out, leaves, g))
+    for i, leaf in enumerate(leaves):   # one at a time
+        rest = [x if j == i else x.detach() for j, x in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(run(*rest), leaf, g)[0], want[i])
+    with torch.no_grad():
+        assert not run(*leaves).requires_grad
+    assert not run(*[x.detach() for x in leaves]).requires_grad
+    a, _ = qk_norm_rotary(leaves[0], leaves[1])
+    assert not torch.autograd.grad(a.sum(), leaves[1])[0].any()   # the other output's gradient counts as zeros
+    out = run(*leaves)
+    with torch.no_grad():
+        leaves[2].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, leaves, g)
+
+
+def test_differentiated_again_is_refused(device):
+    leaves, run = _both(device)
+    first = torch.autograd.grad(run(*leaves).sum(), leaves, create_graph=True)
+    assert all(x.requires_grad for x in first)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first[0].sum(), leaves[0])
+
+
+def test_backward_in_other_threads_and_on_a_stream(device):
+    leaves, run = _both(device, torch.bfloat16)
+    out = run(*leaves)
+    g = torch.ones_like(out)
+    want = torch.autograd.grad(out, leaves, g)
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = torch.autograd.grad(run(*leaves), leaves, g)
+            torch.cuda.current_stream().synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, y) for run_ in got for x, y in zip(run_, want))
+
+
+def test_out_of_memory_is_torchs(device):
+    q = torch.zeros(1 << 20, 8, 32, device=device)   # 1 GiB; its outputs as much again
+    cu = torch.tensor([0, 10], dtype=torch.int32, device=device)
+    bias = torch.zeros(8, 8, device=device)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_allocated() + (256 << 20)) / torch.cuda.mem_get_info()[1])
+    try:
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            relative_attention(q, q, q, bias, cu, cu, max_distance=20)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            qk_norm_rotary(q)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert not relative_attention(q[:64], q[:64], q[:64], bias, cu, cu, max_distance=20).any()
