@@ -2083,7 +2083,7 @@ __global__ __launch_bounds__(f32_threads(HD, TOK)) __attribute__((amdgpu_waves_p
   };
   walk(std::false_type());
   if (BIAS)
-    rel_fold<T::kThreads>(sRel, sums, a.rel, a.rel.part + ((size_t)a.rel.slot[item] * H + head) * a.rel.buckets, wave, lane, tid);
+    rel_fold<T::kThreads>(sRel, sums, a.rel, a.rel.part + ((size_t)rel_place(a.rel, item, a.plan[item].x) * H + head) * a.rel.buckets, wave, lane, tid);
   if (MASKED && __syncthreads_or(odd)) {   // again, over the admissible pairs alone
 #pragma unroll
     for (int b = 0; b < QB; ++b)

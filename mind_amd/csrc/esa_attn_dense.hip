@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256) ESA_WAVES_ATTR(BIAS ? 4 : ESA_DENSE_WAVES_DQ) 
   });
   if (BIAS) {
     far_done();
-    rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)a.rel.slot[item] * H + head) * a.rel.buckets, wave, lane, tid);
+    rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)rel_place(a.rel, item, g.x) * H + head) * a.rel.buckets, wave, lane, tid);
   }
 #pragma unroll
   for (int u = 0; u < T; ++u)

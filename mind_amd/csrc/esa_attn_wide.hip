@@ -686,7 +686,7 @@ void wide_dq_kernel(const WideArgs a) {
         }
         if (BIAS && near) sums.stage32(kept[0], kept[1], base, lane);
       });
-  if (BIAS) rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)a.rel.slot[item] * H + head) * a.rel.buckets, wave, lane, tid);
+  if (BIAS) rel_fold<256>(sRel, sums, a.rel, a.rel.part + ((size_t)rel_place(a.rel, item, g.x) * H + head) * a.rel.buckets, wave, lane, tid);
   if (!valid) return;
   store_acc<HD>(a.dq + ((size_t)t * H + head) * HD, acc, a.scale, h);
 }

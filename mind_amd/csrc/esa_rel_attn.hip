@@ -61,7 +61,7 @@ int group_tokens(int batch, int total_q, int total_k, int heads, int head_dim, i
 
 // The bf16 forward of few queries (at most 32 a segment on average) over many keys (512 and more): with a block per
 // segment and head at most kSplitMaxSegments blocks walk all of a segment's keys, one of their waves at work.  Cut so
-// that about 2,048 blocks have `keys` each, 16 protein graphs (68,000 keys, 16 heads of 32), three queries each, take
+// that about 2,048 blocks have `keys` each, 16 protein graphs (20,364 keys, 16 heads of 32), three queries each, take
 // 14 us and 7 to join them instead of 31.
 int split_keys(int batch, int total_q, int total_k, int heads, int dtype, bool backward) {
   if (backward || dtype != ESA_BF16 || total_q == 0 || total_q > (long long)kSplitRows * batch || batch > kSplitMaxSegments ||
@@ -75,7 +75,7 @@ size_t split_most(int batch, int total_q, int total_k, int keys) {
   return (size_t)(total_q + kSplitRows - 1) / kSplitRows + (size_t)(total_k + keys - 1) / keys + 2 * (size_t)batch;
 }
 
-struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, first_q, slot_q, line, top, ranges, knorm, rows, part, where, acc, ml, total; };
+struct Layout { size_t counts, plan_q, plan_k, shift_q, shift_k, first_q, segment_q, line, top, ranges, knorm, rows, part, where, acc, ml, total; };
 Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int buckets, int reach, int dtype, bool backward) {
   Layout w{};
   size_t off = 0;
@@ -99,7 +99,7 @@ Layout layout(int batch, int total_q, int total_k, int heads, int head_dim, int 
     w.plan_k = take(gk * sizeof(int4));
     w.shift_k = take(gk * sizeof(int));
     w.first_q = take((size_t)batch * sizeof(int));
-    w.slot_q = take(gq * sizeof(int));
+    w.segment_q = take(gq * sizeof(int));
     w.rows = take((size_t)heads * tiles32(total_q) * kTile * sizeof(float2));
     w.part = take(gq * heads * buckets * sizeof(float));
   } else if (dtype == ESA_BF16) {
@@ -159,7 +159,9 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
     r.plan_k = reinterpret_cast<int4*>(at(w.plan_k));
     r.shift_k = reinterpret_cast<int*>(at(w.shift_k));
     r.first_q = reinterpret_cast<int*>(at(w.first_q));
-    r.bias.slot = r.slot_q = reinterpret_cast<int*>(at(w.slot_q));
+    r.bias.segment = r.segment_q = reinterpret_cast<int*>(at(w.segment_q));
+    r.bias.first = r.first_q;
+    r.bias.cu = c.cu_q;
     r.rows = reinterpret_cast<float2*>(at(w.rows));
   } else if (dtype == ESA_BF16) {
     if ((r.split.keys = split_keys(c.nseg, c.total_q, c.total_k, c.heads, dtype, false))) {
@@ -182,7 +184,7 @@ void fill(const Layout& w, char* ws, const void* table, int table_dtype, int buc
   p.zero_k = static_cast<uint4*>(c.dk); p.zero_v = static_cast<uint4*>(c.dv);
   p.lse = backward ? nullptr : c.lse;
   p.backward = backward;
-  p.gtok_q = p.gtok_k = r.group_tok = group_tokens(c.nseg, c.total_q, c.total_k, c.heads, c.head_dim, dtype);
+  p.gtok_q = p.gtok_k = r.group_tok = r.bias.tok = group_tokens(c.nseg, c.total_q, c.total_k, c.heads, c.head_dim, dtype);
   p.key_pairs = backward && c.dropout && dtype == ESA_BF16;   // the bf16 dK/dV pass shares its hashes by key pairs
 }
 

@@ -54,7 +54,10 @@ struct RelBias {
   int reach, stride;        // stride = 2 (reach + kRelPad) + 1
   int buckets, far_lo, far_hi;   // the buckets of d <= -reach and d >= reach
   float* part;              // dQ pass: [groups][heads][buckets], the groups in their tokens' order
-  const int* slot;          // dQ pass: a listed group's place in that order
+  const int* segment;       // dQ pass: a listed group's segment,
+  const int* first;         // that segment's first place in that order
+  const int* cu;            // and its first token;
+  int tok;                  // tokens of a group
 };
 
 // Few queries over many keys (bf16 forward): a group is 32 queries of one
@@ -82,7 +85,7 @@ struct RelPass {
   int4* plan_q; int4* plan_k;       // groups of 128 or 64 tokens (seg_plan_block); plan_k backward only
   int* count_q; int* count_k;
   int* shift_q; int* shift_k;       // per group: d = key token - query token - shift
-  int* first_q; int* slot_q;        // backward: a segment's first place, a listed group's place in the tokens' order
+  int* first_q; int* segment_q;     // backward: RelBias's first and segment
   float* knorm; int tk_tiles;       // bf16 forward: max |k| per (head, 32-key tile)
   float2* rows; int tq_pad;         // backward: row statistics [heads][tq_pad]
   RelSplit split;                   // bf16 forward of few queries
@@ -101,7 +104,7 @@ struct RelPrep {
   int gtok_q, gtok_k;                                               // tokens of a group of queries, of keys
 };
 constexpr int kRelClearBlocks = 16;
-inline int rel_prep_blocks(const RelPrep& p) { return 1 + (p.backward ? 1 : 0) + p.heads + kRelClearBlocks; }
+inline int rel_prep_blocks(const RelPrep& p) { return 1 + (p.backward ? 2 : 0) + p.heads + kRelClearBlocks; }
 
 // esa_attn_dense.hip (bf16: its own kernels at head dim 16 without dropout, else the next file's), esa_attn_wide.hip,
 // esa_attn.hip (fp32).
@@ -281,12 +284,27 @@ DEVI int rel_bucket(const RelPrep& p, int d) {
   return lo + (p.two_sided && d > 0 ? p.side : 0);
 }
 
+// Exclusive sums over 256 threads.
+DEVI int before_me(int x, int tid) {
+  __shared__ int waves[4];
+  int sum = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(sum, o);
+    if ((tid & 63) >= o) sum += y;
+  }
+  if ((tid & 63) == 63) waves[tid >> 6] = sum;
+  __syncthreads();
+  for (int w = 0; w < tid >> 6; ++w) sum += waves[w];
+  return sum - x;
+}
+
 // The groups of a split forward (at most kSplitMaxSegments segments), in order.
 template <class ShiftOf>
 DEVI void split_plan_block(const RelPrep& p, const RelPass& r, int tid, ShiftOf shift_of) {
   constexpr int PER = kSplitMaxSegments / 256;
   __shared__ int first[kSplitMaxSegments + 1];
-  __shared__ int part[256];
+  __shared__ int all;
   int loc[PER], sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -297,26 +315,18 @@ DEVI void split_plan_block(const RelPrep& p, const RelPass& r, int tid, ShiftOf 
       sum += n.x * n.y;
     }
   }
-  part[tid] = sum;
-  __syncthreads();
-  for (int off = 1; off < 256; off <<= 1) {
-    const int add = tid >= off ? part[tid - off] : 0;
-    __syncthreads();
-    part[tid] += add;
-    __syncthreads();
-  }
-  const int base = part[tid] - sum;
+  const int base = before_me(sum, tid);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int s = tid * PER + i;
     first[s] = base + loc[i];
   }
   if (tid == 255) {
-    first[kSplitMaxSegments] = part[255];
-    *r.count_q = part[255];
+    all = first[kSplitMaxSegments] = base + sum;
+    *r.count_q = base + sum;
   }
   __syncthreads();
-  for (int e = tid; e < part[255]; e += 256) {
+  for (int e = tid; e < all; e += 256) {
     int lo = 0, hi = p.nseg;   // the last segment that begins at or before e: it is not empty
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -336,25 +346,20 @@ DEVI void split_plan_block(const RelPrep& p, const RelPass& r, int tid, ShiftOf 
 // first[s] = groups of the segments before s.  The plan lists groups of equal work in any order; the table's partial sums
 // are added in this one.
 DEVI void seg_first_block(const int* cu, int nseg, int gtok, int* first, int tid) {
-  __shared__ int part[256];
   const int per = (nseg + 255) / 256, s0 = min(tid * per, nseg), s1 = min(s0 + per, nseg);
   auto groups = [&](int s) { return max(cu[s + 1] - cu[s] + gtok - 1, 0) / gtok; };
   int sum = 0;
   for (int s = s0; s < s1; ++s) sum += groups(s);
-  part[tid] = sum;
-  __syncthreads();
-  for (int off = 1; off < 256; off <<= 1) {
-    const int add = tid >= off ? part[tid - off] : 0;
-    __syncthreads();
-    part[tid] += add;
-    __syncthreads();
-  }
-  int at = part[tid] - sum;
+  int at = before_me(sum, tid);
   for (int s = s0; s < s1; ++s) {
     first[s] = at;
     at += groups(s);
   }
-  __syncthreads();
+}
+// The place of listed group `item`, which begins at token x.
+DEVI int rel_place(const RelBias& r, int item, int x) {
+  const int s = r.segment[item];
+  return r.first[s] + (x - r.cu[s]) / r.tok;
 }
 
 // Block b of the preparation's rel_prep_blocks (256 threads).
@@ -368,10 +373,9 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
     return;
   }
   if (b == 0) {
-    if (p.backward) seg_first_block(p.cu_q, p.nseg, p.gtok_q, r.first_q, tid);
-    seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, [&](int i, int s, int j) {
+    seg_plan_block(p.cu_q, p.cu_k, p.nseg, p.gtok_q, r.plan_q, r.count_q, tid, false, [&](int i, int s, int) {
       r.shift_q[i] = shift_of(s);
-      if (p.backward) r.slot_q[i] = r.first_q[s] + j;
+      if (p.backward) r.segment_q[i] = s;
     });
     return;
   }
@@ -382,7 +386,11 @@ DEVI void rel_prep_block(const RelPrep& p, const RelPass& r, int b, int tid) {
                      [&](int i, int s, int) { r.shift_k[i] = shift_of(s); });
       return;
     }
-    b -= 1;
+    if (b == 1) {
+      seg_first_block(p.cu_q, p.nseg, p.gtok_q, r.first_q, tid);
+      return;
+    }
+    b -= 2;
   }
   if (b < p.heads) {   // one head's line
     __shared__ float most[4];
