@@ -66,7 +66,8 @@ def _build_tensors() -> None:
     src, tmp = CSRC / "esa_tensors.cpp", TENSORS.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
-           *(f"-I{p}" for p in include_paths()), "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", str(src), "-o", str(tmp), *(f"-L{p}" for p in library_paths()),
+           *(f"-I{p}" for p in include_paths()), f"-I{Path(hipcc()).resolve().parent.parent / 'include'}",
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", str(src), "-o", str(tmp), *(f"-L{p}" for p in library_paths()),
            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]   # torch has loaded them by the time this module is
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
