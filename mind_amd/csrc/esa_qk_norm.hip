@@ -371,7 +371,9 @@ int esa_qk_norm_bwd(const void* gq, const void* gk, const void* q, const void* k
   esa_qk_norm_bwd_workspace_size(total, head_dim, &need);
   if (total > 0) {
     if (!gq || !dq || (heads_k && (!gk || !dk)) || (weights && !workspace)) return ESA_ERR_NULL;
-    if (off_boundary(gq) || off_boundary(gk) || off_boundary(dq) || off_boundary(dk)) return ESA_ERR_ALIGN;
+    if (off_boundary(gq) || off_boundary(gk) || off_boundary(dq) || off_boundary(dk) ||
+        (weights && reinterpret_cast<uintptr_t>(workspace) % alignof(float)))
+      return ESA_ERR_ALIGN;
     if (weights && workspace_bytes < need) return ESA_ERR_WORKSPACE;
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

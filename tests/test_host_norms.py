@@ -65,6 +65,7 @@ def test_qk_norm_entry_points_refuse_before_launch():
         return lib.esa_qk_norm_bwd(gq, 16, 16, 16, s, 5, 2, 2, 16, 0, None, None, None, 0, None, 0, 0, 0.0, dq, 16, dwq, None, ws,
                                    nbytes, None)
     assert bwd(gq=None) == -1 and bwd(dq=None) == -1 and bwd(ws=None) == -1 and bwd(nbytes=4) == -4 and bwd(gq=4) == -6
+    assert bwd(ws=18) == -6
 
 
 def test_gradient_norm_refuses_host_tensors():
