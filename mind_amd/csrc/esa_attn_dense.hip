@@ -905,7 +905,11 @@ static DenseArgs dense_rel_args(const DenseAttnCall& c, const RelPass& r) {
 }
 
 int dense_rel_fwd(const DenseAttnCall& c, const RelPass& r, RelPrep p, hipStream_t st) {
-  if (c.head_dim != kHd || c.dropout || r.split.keys) return wide_rel_fwd(c, r, p, st);
+  // With few blocks the walk of the longest segment is the time, and the other forward's waves take one query tile of 32
+  // through it, these two.  Molecules, us here -> there by blocks of 128 queries: 8 heads, 184 blocks 21.1 -> 15.8, 912: 25.3
+  // -> 22.4, 1,872: 31.7 -> 32.9; 32 heads, 736: 22.1 -> 18.6, 1,504: 25.9 -> 29.3, 7,488: 87 -> 99.
+  const bool few = ((long long)(c.total_q + kGroupTok - 1) / kGroupTok + min(c.nseg, c.total_q)) * c.heads <= 1024;
+  if (c.head_dim != kHd || c.dropout || r.split.keys || few) return wide_rel_fwd(c, r, p, st);
   p.gtok_q = kFwdGroup;
   const int nb = rel_prep_blocks(p);
   ESA_TIMED(esa_profile::kAttnPrep, st,

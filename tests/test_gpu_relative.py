@@ -476,3 +476,31 @@ def test_table_gradient_of_many_equal_segments(device, dtype, hd):
 def test_blocks_between_in_single_precision(device, hd, dropout):
     """The fp32 kernels' groups of 64 tokens with more blocks than the forward's halved walk takes."""
     check(device, torch.float32, 7, hd, [100] * 150, dropout=dropout, seed=67)
+
+
+MANY = [1, 31, 32, 33, 64, 65] * 12 + [300, 0, 257, 512]   # with 16 heads more than 1,024 blocks
+
+
+@pytest.mark.parametrize("change", [None, lambda b: b * 30, lambda b: torch.where(b > 1.0, torch.full_like(b, -math.inf), b),
+                                    lambda b: b.index_fill(1, torch.tensor([3, 7], device=b.device), -math.inf)],
+                         ids=["plain", "wide", "left out", "heads left out"])
+def test_many_blocks_at_head_dim_16(device, change):
+    """The bf16 forward of many blocks (few take the other head dims' kernel)."""
+    check(device, torch.bfloat16, 16, 16, MANY, seed=101, extra=5, bias=change, peaked=change is not None)
+
+
+def test_many_blocks_at_head_dim_16_of_chunks(device):
+    lens_q = [max(n - 20, 0) for n in MANY]
+    check(device, torch.bfloat16, 24, 16, lens_q, MANY, starts=[n - m for n, m in zip(MANY, lens_q)], seed=103)
+
+
+def test_many_blocks_at_head_dim_16_beside_what_is_not_finite(device):
+    q, k, v, _, b, cu, _ = case(device, torch.bfloat16, 16, 16, MANY, seed=105)
+    want = relative_attention(q, k, v, b, cu, cu)
+    bad = slice(int(cu[40]), int(cu[41]))
+    k[bad], v[bad] = math.nan, math.inf
+    got = relative_attention(q, k, v, b, cu, cu)
+    rest = torch.ones(q.shape[0], dtype=torch.bool, device=device)
+    rest[bad] = False
+    # key norms are by 32 tokens of the whole tensor: the neighbours' softmax may take another reference point
+    assert rel_err(got[rest], want[rest].double().cpu()) <= 6e-3 and bool(torch.isnan(got[bad]).all())
